@@ -125,9 +125,54 @@ VEC_SYMBOLS = [
 ]
 
 
-def bind(cdll):
-    """Attach prototypes for every declared symbol (both headers); raises AttributeError if one is missing."""
-    for name, res, args in SYMBOLS + VEC_SYMBOLS:
+# ---- include/agarcl_learn.h: what a learner runs around the vector step -----------------------------------------------------------
+F32, BF16, F16 = 0, 1, 2
+MARK_STEPS = 8       # AGARCL_MARK_STEPS
+
+
+def _fields(text):
+    """"p x, i64 n": ctypes fields of a structure of the header, in its order"""
+    kinds = {"p": C.c_void_p, "i64": C.c_int64, "i32": C.c_int32, "f32": C.c_float}
+    return [(name, kinds[k]) for k, name in (f.split() for f in text.split(","))]
+
+
+class RecurrenceArgs(C.Structure):
+    _fields_ = _fields("i64 steps, i64 rows, i64 width, i32 dtype, i32 device, p x, p gate, i64 x_stride, i64 gate_stride, p state, p reset, i64 reset_stride, p h, p last, "
+                       "p marks, p dh, i64 dh_stride, p dlast, p dx, p dgate, p dstate, p work, p stream")
+
+
+class AdvantagesArgs(C.Structure):
+    _fields_ = _fields("i64 steps, i64 rows, i32 dtype, i32 device, p reward, p value, p next_value, p terminated, p truncated, p final_value, i64 reward_stride, "
+                       "i64 value_stride, i64 terminated_stride, i64 truncated_stride, i64 final_stride, f32 gamma, f32 lambda, p advantage, p returns, p work, p stream")
+
+
+class SampleArgs(C.Structure):
+    _fields_ = _fields("i64 rows, i64 kinds, i32 dtype, i32 device, p logits, i64 logits_stride, p allowed, i64 allowed_stride, p gumbel, i64 gumbel_stride, p mean, p log_std, "
+                       "i32 log_std_per_row, i32 reserved, p normal, p kind, p log_prob, p raw, p move, p stream")
+
+
+class PolicyLossArgs(C.Structure):
+    _fields_ = _fields("i64 rows, i64 kinds, i32 dtype, i32 device, p logits, i64 logits_stride, p allowed, i64 allowed_stride, p kind, p mean, p log_std, i32 log_std_per_row, "
+                       "i32 mean_over_weight, p move, p old_log_prob, p advantage, p ref_log_prob, p weight, p weight_sum, f32 clip_low, f32 clip_high, f32 kl_coef, f32 entropy_coef, "
+                       "p upstream, i32 skip_if_one, i32 want_stats, p loss, p stats, p dlogits, p dmean, p dlog_std, p dlog_std_one, p work, p stream")
+
+
+LEARN_SYMBOLS = [
+    ("agarcl_learn_error", C.c_char_p, []),
+    ("agarcl_recurrence_work", C.c_int64, [C.c_int64, C.c_int64, C.c_int64]),
+    ("agarcl_recurrence", C.c_int, [C.POINTER(RecurrenceArgs)]),
+    ("agarcl_recurrence_grad", C.c_int, [C.POINTER(RecurrenceArgs)]),
+    ("agarcl_advantages_work", C.c_int64, [C.c_int64, C.c_int64]),
+    ("agarcl_advantages", C.c_int, [C.POINTER(AdvantagesArgs)]),
+    ("agarcl_sample_actions", C.c_int, [C.POINTER(SampleArgs)]),
+    ("agarcl_policy_loss_work", C.c_int64, []),
+    ("agarcl_policy_loss", C.c_int, [C.POINTER(PolicyLossArgs)]),
+]
+
+
+def bind(cdll, symbols=SYMBOLS + VEC_SYMBOLS):
+    """Attach prototypes for every declared symbol (of the engine's two headers by default); raises AttributeError if one is missing."""
+    for name, res, args in symbols:
         fn = getattr(cdll, name)
         fn.restype = res
         fn.argtypes = args
@@ -149,7 +194,7 @@ def hip_lib():
         if not os.path.exists(HIP_SO):
             raise AgarclError(-4, "HIP extension %s is missing -- build it with agarcl_amd/build.py "
                                   "(there is no CPU fallback)" % HIP_SO)
-        _hip = bind(C.CDLL(HIP_SO))
+        _hip = bind(bind(C.CDLL(HIP_SO)), LEARN_SYMBOLS)
     return _hip
 
 

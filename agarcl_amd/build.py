@@ -8,7 +8,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, "csrc", "agar_engine.hip")
 import glob
 # every file under csrc/ is a dependency (one translation unit that #includes the .inl / .h files)
-DEPS = sorted(glob.glob(os.path.join(HERE, "csrc", "*"))) + [os.path.join(HERE, "..", "include", h) for h in ("agarcl_batch.h", "agarcl_vec.h")]
+# the learner's operators (include/agarcl_learn.h): a unit of their own, so that the engine's source and its profiles do not depend on them
+LEARN_SRC = os.path.join(HERE, "csrc_learn", "agar_learn.hip")
+DEPS = (sorted(glob.glob(os.path.join(HERE, "csrc", "*"))) + sorted(glob.glob(os.path.join(HERE, "csrc_learn", "*")))
+        + [os.path.join(HERE, "..", "include", h) for h in ("agarcl_batch.h", "agarcl_vec.h", "agarcl_learn.h")])
 OUT = os.path.join(HERE, "libagarcl_hip.so")
 
 FLAGS = [
@@ -16,6 +19,10 @@ FLAGS = [
     # bit-exact fp32 vs the reference's x86-64 build: no FMA contraction, IEEE divide / sqrt
     "-ffp-contract=off", "-fhip-fp32-correctly-rounded-divide-sqrt", "-fno-fast-math",
 ]
+# hipcc -O3 turns ordinary float code into packed f32 instructions, some forms of which have given wrong results on this hardware
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# the learner's operators are compared with 64-bit results within tolerances, not bit for bit: FMAs are welcome
+LEARN_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=fast", "-fno-fast-math"] + NO_PACKED_F32
 
 
 def hipcc():
@@ -48,8 +55,8 @@ def _compile(args):
 
 
 def build(force=False, verbose=False, extra=(), out=OUT, single=False, jobs=None):
-    """Seventeen translation units compiled in parallel -- the main unit (-DAG_SPLIT_BUILD: host code, C ABI, observation kernels) and two
-    part units per (NS, AV) pair (-DAG_PART_NS / -DAG_PART_AV / -DAG_PART_KIND: the step or the front kernels of that pair, agar_engine.hip
+    """Eighteen translation units compiled in parallel -- the main unit (-DAG_SPLIT_BUILD: host code, C ABI, observation kernels), the learner's
+    operators (csrc_learn/) and two part units per (NS, AV) pair (-DAG_PART_NS / -DAG_PART_AV / -DAG_PART_KIND: the step or the front kernels of that pair, agar_engine.hip
     "split build") -- linked into one shared library.  single=True compiles the same source as one unit (3-4 minutes instead of < 1).
     extra/out: diagnostic variants only (e.g. -DAGAR_PROFILE -> build_variants/lib_PROF.so, used by scripts/; build_variants/ is
     git-ignored and travels to the GPU box only while it exists -- delete it when the measurements are done)."""
@@ -59,13 +66,14 @@ def build(force=False, verbose=False, extra=(), out=OUT, single=False, jobs=None
     if verbose:
         base.insert(1, "-Rpass-analysis=kernel-resource-usage")
     if single or os.environ.get("AGARCL_BUILD_SINGLE") == "1":   # (one unit: STEP_FLAGS would then reach the front kernels too, so they are left out)
-        subprocess.check_call(base + ["-o", out, SRC])
+        subprocess.check_call(base + ["-o", out, SRC, LEARN_SRC])
         return out
     import tempfile
     from concurrent.futures import ThreadPoolExecutor
     comp = [f for f in base if f != "-shared"]
     with tempfile.TemporaryDirectory(prefix="agarcl_build_") as tmp:
-        units = [comp + ["-DAG_SPLIT_BUILD", "-c", SRC, "-o", os.path.join(tmp, "main.o")]]
+        units = [comp + ["-DAG_SPLIT_BUILD", "-c", SRC, "-o", os.path.join(tmp, "main.o")],
+                 [hipcc()] + LEARN_FLAGS + list(extra) + (["-Rpass-analysis=kernel-resource-usage"] if verbose else []) + ["-c", LEARN_SRC, "-o", os.path.join(tmp, "learn.o")]]
         for ns, av, kind in PARTS:
             units.append(comp + (STEP_FLAGS if kind == 0 else []) + ["-DAG_PART_NS=%d" % ns, "-DAG_PART_AV=%d" % av, "-DAG_PART_KIND=%d" % kind, "-c", SRC,
                                  "-o", os.path.join(tmp, "part_%d_%d_%d.o" % (ns, av, kind))])
