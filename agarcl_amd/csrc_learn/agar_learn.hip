@@ -4,9 +4,11 @@
 #include <math.h>
 #include <stdint.h>
 #include <string>
+#include <type_traits>
 
 #include "../../include/agarcl_learn.h"
 #include "learn_common.inl"
+#include "learn_scan.inl"
 #include "learn_recurrence.inl"
 #include "learn_policy.inl"
 
@@ -25,7 +27,8 @@ struct DeviceScope {
 };
 #define ON_DEVICE(dev) DeviceScope scope_(dev); if (scope_.err != hipSuccess) return fail(AGARCL_E_HIP, "device", hipGetErrorString(scope_.err))
 static int launched(const char *what) { const hipError_t e = hipGetLastError(); return e == hipSuccess ? AGARCL_OK : fail(AGARCL_E_HIP, what, hipGetErrorString(e)); }
-#define BY_TYPE(dt, CALL) do { switch (dt) { case AGARCL_F32: { using T = float; CALL; break; } case AGARCL_BF16: { using T = bf16_t; CALL; break; } default: { using T = f16_t; CALL; break; } } } while (0)
+#define BY_TYPE(dt, ...) do { switch (dt) { case AGARCL_F32: { using T = float; __VA_ARGS__; break; } case AGARCL_BF16: { using T = bf16_t; __VA_ARGS__; break; } default: { using T = f16_t; __VA_ARGS__; break; } } } while (0)
+#define BY_VEC(vec, WIDE, ...) do { if ((vec) == WIDE) { constexpr int V = WIDE; __VA_ARGS__; } else { constexpr int V = 1; __VA_ARGS__; } } while (0)
 static bool type_ok(int32_t dt) { return dt == AGARCL_F32 || dt == AGARCL_BF16 || dt == AGARCL_F16; }
 static const int64_t kMost = (int64_t)1 << 40;      // no dimension, stride or product of dimensions above this: 64-bit index arithmetic cannot overflow
 static bool sizes_ok(int64_t a, int64_t b, int64_t c) {
@@ -37,7 +40,7 @@ static bool stride_ok(int64_t s, int64_t steps, int64_t least) { return steps <=
 static unsigned blocks_for(int64_t threads) { const int64_t n = (threads + 255) / 256; return (unsigned)(n < 65536 ? n : 65536); }   // (the kernels go on in strides of the grid)
 
 // ---- recurrence -----------------------------------------------------------------------------------------------------------------------------
-extern "C" int64_t agarcl_recurrence_work(int64_t steps, int64_t rows, int64_t width) { return sizes_ok(steps, rows, width) ? 0 : -1; }
+extern "C" int64_t agarcl_recurrence_work(int64_t steps, int64_t rows, int64_t width) { return sizes_ok(steps, rows, width) ? scan_work(steps, rows * width) : -1; }
 
 static int recurrence_check(const agarcl_recurrence_args *a) {
   if (!a) return fail(AGARCL_E_INVALID, "null argument");
@@ -59,8 +62,18 @@ extern "C" int agarcl_recurrence(const agarcl_recurrence_args *a) {
   if (!a->last || (a->steps && !a->h)) return fail(AGARCL_E_INVALID, "h, last");
   ON_DEVICE(a->device);
   const hipStream_t st = (hipStream_t)a->stream;
-  BY_TYPE(a->dtype, (k_recurrence<T><<<dim3(blocks_for(k)), 256, 0, st>>>((const T *)a->x, (const T *)a->gate, a->x_stride, a->gate_stride, a->state, a->reset,
-      a->reset_stride, (T *)a->h, a->last, a->marks, a->steps, a->rows, a->width)));
+  if (a->steps == 0) {      // (the state as it is)
+    k_copy_state<<<dim3(blocks_for(k)), 256, 0, st>>>(a->state, a->last, k);
+  } else BY_TYPE(a->dtype, {
+    constexpr int wide = 4;
+    const ScanPlan p = scan_plan(a->steps, k, wide);
+    BY_VEC(p.vec, wide, {
+    RecurrenceOp<T, V> op;
+    op.x = (const T *)a->x; op.gate = (const T *)a->gate; op.xs = a->x_stride; op.gs = a->gate_stride; op.reset = a->reset; op.rs = a->reset_stride; op.h = (T *)a->h;
+    op.marks = a->marks; op.steps = a->steps; op.columns = k; op.width = a->width;
+    scan_launch<RecurrenceOp<T, V>, V>(op, p.sh, a->state, a->last, a->work, st);
+    });
+  });
   return launched("recurrence");
 }
 
@@ -72,13 +85,23 @@ extern "C" int agarcl_recurrence_grad(const agarcl_recurrence_args *a) {
   if (a->steps && a->dh && !stride_ok(a->dh_stride, a->steps, k)) return fail(AGARCL_E_INVALID, "a stride is smaller than a step");
   ON_DEVICE(a->device);
   const hipStream_t st = (hipStream_t)a->stream;
-  BY_TYPE(a->dtype, (k_recurrence_grad<T><<<dim3(blocks_for(k)), 256, 0, st>>>((const T *)a->x, (const T *)a->gate, a->x_stride, a->gate_stride, a->reset,
-      a->reset_stride, a->marks, (const T *)a->dh, a->dh_stride, a->dlast, (T *)a->dx, (T *)a->dgate, a->dstate, a->steps, a->rows, a->width)));
+  if (a->steps == 0) {
+    k_copy_state<<<dim3(blocks_for(k)), 256, 0, st>>>(a->dlast, a->dstate, k);
+  } else BY_TYPE(a->dtype, {
+    constexpr int wide = sizeof(T) == 4 ? 2 : 4;
+    const ScanPlan p = scan_plan(a->steps, k, wide);
+    BY_VEC(p.vec, wide, {
+    RecurrenceGradOp<T, V> op;
+    op.x = (const T *)a->x; op.gate = (const T *)a->gate; op.dh = (const T *)a->dh; op.xs = a->x_stride; op.gs = a->gate_stride; op.ds = a->dh_stride; op.reset = a->reset;
+    op.rs = a->reset_stride; op.marks = a->marks; op.dx = (T *)a->dx; op.dgate = (T *)a->dgate; op.steps = a->steps; op.columns = k; op.width = a->width;
+    scan_launch<RecurrenceGradOp<T, V>, V>(op, p.sh, a->dlast, a->dstate, a->work, st);
+    });
+  });
   return launched("recurrence gradient");
 }
 
 // ---- advantages -----------------------------------------------------------------------------------------------------------------------------
-extern "C" int64_t agarcl_advantages_work(int64_t steps, int64_t rows) { return sizes_ok(steps, rows, 1) ? 0 : -1; }
+extern "C" int64_t agarcl_advantages_work(int64_t steps, int64_t rows) { return sizes_ok(steps, rows, 1) ? scan_work(steps, rows) : -1; }
 
 extern "C" int agarcl_advantages(const agarcl_advantages_args *a) {
   if (!a) return fail(AGARCL_E_INVALID, "null argument");
@@ -94,9 +117,14 @@ extern "C" int agarcl_advantages(const agarcl_advantages_args *a) {
   if (agarcl_advantages_work(a->steps, a->rows) > 0 && !a->work) return fail(AGARCL_E_INVALID, "work");
   ON_DEVICE(a->device);
   const hipStream_t st = (hipStream_t)a->stream;
-  BY_TYPE(a->dtype, (k_advantages<T><<<dim3(blocks_for(a->rows)), 256, 0, st>>>(a->reward, (const T *)a->value, (const T *)a->next_value, a->terminated, a->truncated,
-      (const T *)a->final_value, a->reward_stride, a->value_stride, a->terminated_stride, a->truncated_stride, a->final_stride, a->gamma, a->gamma * a->lambda, a->advantage,
-      a->returns, a->steps, a->rows)));
+  const ScanPlan p = scan_plan(a->steps, a->rows, 4);
+  BY_TYPE(a->dtype, BY_VEC(p.vec, 4, {
+    AdvantageOp<T, V> op;
+    op.reward = a->reward; op.value = (const T *)a->value; op.next_value = (const T *)a->next_value; op.terminated = a->terminated; op.truncated = a->truncated;
+    op.final_value = (const T *)a->final_value; op.rs = a->reward_stride; op.vs = a->value_stride; op.es = a->terminated_stride; op.us = a->truncated_stride; op.fs = a->final_stride;
+    op.gamma = a->gamma; op.gl = a->gamma * a->lambda; op.advantage = a->advantage; op.returns = a->returns; op.steps = a->steps; op.columns = a->rows;
+    scan_launch<AdvantageOp<T, V>, V>(op, p.sh, nullptr, nullptr, a->work, st);
+  }));
   return launched("advantages");
 }
 
