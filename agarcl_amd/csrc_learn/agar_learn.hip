@@ -147,8 +147,7 @@ extern "C" int agarcl_sample_actions(const agarcl_sample_args *a) {
   if (a->gumbel && !stride_ok(a->gumbel_stride, a->rows, a->kinds)) return fail(AGARCL_E_INVALID, "a stride is smaller than a row");
   if (a->mean ? (!a->log_std || !a->raw || !a->move) : (a->log_std || a->normal)) return fail(AGARCL_E_INVALID, "mean, log_std, raw, move belong together");
   ON_DEVICE(a->device);
-  const unsigned grid = (unsigned)((a->rows + 3) / 4 < 65536 ? (a->rows + 3) / 4 : 65536);
-  BY_TYPE(a->dtype, (k_sample<T><<<dim3(grid), 256, 0, (hipStream_t)a->stream>>>(*a)));
+  BY_TYPE(a->dtype, sample_launch<T>(*a, (hipStream_t)a->stream));
   return launched("sample_actions");
 }
 
@@ -172,13 +171,13 @@ extern "C" int agarcl_policy_loss(const agarcl_policy_loss_args *a) {
     k_weight_sum<<<dim3(kWeightBlocks), 256, 0, st>>>(a->weight, a->rows, a->work + 8 * kLossBlocks);
     if (const int rc = launched("policy loss: weights")) return rc;
   }
-  unsigned grid = (unsigned)((a->rows + 3) / 4 < kLossBlocks ? (a->rows + 3) / 4 : kLossBlocks);
-  if (grid) {
-    BY_TYPE(a->dtype, (k_policy_loss<T><<<dim3(grid), 256, 0, st>>>(*a)));
+  unsigned grid = 0;
+  if (a->rows) {
+    BY_TYPE(a->dtype, grid = loss_launch<T>(*a, st));
     if (const int rc = launched("policy loss")) return rc;
   }
   if (a->want_stats) {
-    k_loss_stats<<<dim3(1), 256, 0, st>>>(*a, (int)grid);
+    k_loss_stats<<<dim3(1), 1024, 0, st>>>(*a, (int)grid);
     if (const int rc = launched("policy loss: sums")) return rc;
   }
   return AGARCL_OK;

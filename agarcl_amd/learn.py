@@ -308,22 +308,36 @@ def _loss_args(logits, mean, log_std, per_row, fixed, kept):
                                 clip_low=clip_low, clip_high=clip_high, kl_coef=kl, entropy_coef=ent, stream=_stream(logits.device))
 
 
-def _loss_forward(logits, mean, log_std, per_row, fixed, std_grad):
-    """(loss, stats, the shared log_std's gradient)"""
+def _loss_forward(logits, mean, log_std, per_row, fixed, std_grad, grads):
+    """(loss, stats, the shared log_std's gradient); grads: the tensors (or None) that take the gradients of logits, mean and a log_std per row in the same pass"""
     L, dev, kept = _capi.hip_lib(), logits.device, []
     a = _loss_args(logits, mean, log_std, per_row, fixed, kept)
     loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(8, dtype=torch.float32, device=dev)
     work = torch.empty(L.agarcl_policy_loss_work(), dtype=torch.float64, device=dev)
     dstd = torch.empty(2, dtype=torch.float32, device=dev) if std_grad else None
-    a.want_stats, a.loss, a.stats, a.work, a.dlog_std = 1, _ptr(loss), _ptr(stats), _ptr(work), _ptr(dstd)
+    a.want_stats, a.loss, a.stats, a.work = 1, _ptr(loss), _ptr(stats), _ptr(work)
+    a.dlogits, a.dmean, a.dlog_std = _ptr(grads[0]), _ptr(grads[1]), _ptr(dstd) if std_grad else _ptr(grads[2])
     _call(L.agarcl_policy_loss, a)
     return loss, stats, dstd
 
 
+def _loss_grads(need, logits, mean, log_std, per_row):
+    like = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)   # noqa: E731
+    return [like(logits) if need[0] else None, like(mean) if need[1] else None, like(log_std) if need[2] and per_row else None]
+
+
 class _PolicyLoss(torch.autograd.Function):
+    """The gradients for an upstream gradient of 1 -- what loss.backward() brings -- are written by the forward pass, from the registers that hold the
+    logits for the loss.  The first backward pass hands them out after its kernel has looked at the upstream gradient: it does nothing where that is
+    1 and works the gradients out from the logits otherwise.  Every other backward pass (a second one through a kept graph, one that is captured: its replays
+    may bring other upstream gradients) works them out, into tensors of its own.  In float16 a loss is scaled as a rule, so there the forward pass leaves them."""
+
     @staticmethod
     def forward(ctx, logits, mean, log_std, per_row, fixed):
-        loss, stats, dstd = _loss_forward(logits, mean, log_std, per_row, fixed, mean is not None and not per_row)
+        need = ctx.needs_input_grad
+        ahead = logits.dtype != torch.float16 and not torch.cuda.is_current_stream_capturing()
+        ctx.ahead = _loss_grads(need, logits, mean, log_std, per_row) if ahead else None
+        loss, stats, dstd = _loss_forward(logits, mean, log_std, per_row, fixed, mean is not None and not per_row, ctx.ahead or (None, None, None))
         ctx.per_row, ctx.numbers = per_row, fixed[7:]
         ctx.save_for_backward(logits, mean, log_std, stats, dstd, *fixed[:7])
         ctx.mark_non_differentiable(stats)
@@ -335,14 +349,16 @@ class _PolicyLoss(torch.autograd.Function):
         L, kept = _capi.hip_lib(), []
         logits, mean, log_std, stats, dstd, *tensors = ctx.saved_tensors
         a = _loss_args(logits, mean, log_std, ctx.per_row, tuple(tensors) + ctx.numbers, kept)
-        need, dev = ctx.needs_input_grad, logits.device
+        need = ctx.needs_input_grad
         upstream = upstream.to(torch.float32).contiguous()
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if need[0] else None
-        dmean = torch.empty(mean.shape, dtype=mean.dtype, device=dev) if need[1] else None
-        dlog = torch.empty(log_std.shape, dtype=log_std.dtype, device=dev) if need[2] else None
-        a.upstream, a.weight_sum, a.dlogits, a.dmean, a.dlog_std, a.dlog_std_one = _ptr(upstream), _ptr(stats) + 16, _ptr(dlogits), _ptr(dmean), _ptr(dlog), _ptr(dstd)
+        grads, ctx.ahead = (None if torch.cuda.is_current_stream_capturing() else ctx.ahead), None
+        a.skip_if_one = int(grads is not None)
+        grads = grads or _loss_grads(need, logits, mean, log_std, ctx.per_row)
+        if need[2] and not ctx.per_row:
+            grads[2] = torch.empty(2, dtype=torch.float32, device=logits.device)
+        a.upstream, a.weight_sum, a.dlogits, a.dmean, a.dlog_std, a.dlog_std_one = _ptr(upstream), _ptr(stats) + 16, _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), _ptr(dstd)
         _call(L.agarcl_policy_loss, a)
-        return dlogits, dmean, dlog, None, None
+        return grads[0], grads[1], grads[2], None, None
 
 
 def policy_loss(logits, kind, old_log_prob, advantage, mean=None, log_std=None, move=None, ref_log_prob=None, allowed=None, weight=None, clip=0.2, kl_coef=0.0,
@@ -389,5 +405,5 @@ def policy_loss(logits, kind, old_log_prob, advantage, mean=None, log_std=None, 
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (logits, mean, log_std)):
         loss, stats = _PolicyLoss.apply(logits, mean, log_std, per_row, fixed)
     else:
-        loss, stats, _ = _loss_forward(logits, mean, log_std, per_row, fixed, False)
+        loss, stats, _ = _loss_forward(logits, mean, log_std, per_row, fixed, False, (None, None, None))
     return PolicyLoss(loss, *stats[:4].unbind())
