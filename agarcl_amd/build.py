@@ -134,6 +134,33 @@ def build_pybind(force=False):
     return out
 
 
+LEARN_TORCH_SRC = os.path.join(HERE, "csrc_learn", "learn_torch.cpp")
+
+
+def learn_torch_out():
+    import sysconfig
+    return os.path.join(HERE, "_learn" + sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+def build_learn_torch(force=False):
+    """g++ -> agarcl_amd/_learn.<abi>.so: torch tensors in and out of include/agarcl_learn.h (csrc_learn/learn_torch.cpp: host only, links the HIP library and
+    torch's own; torch has to be imported before it)."""
+    import sysconfig
+    import torch
+    src, out = LEARN_TORCH_SRC, learn_torch_out()
+    header = os.path.join(HERE, "..", "include", "agarcl_learn.h")
+    if not force and os.path.exists(out) and os.path.getmtime(out) > max(os.path.getmtime(src), os.path.getmtime(header)):
+        return out
+    at = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(hipcc())))
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-DTORCH_EXTENSION_NAME=_learn",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-isystem", os.path.join(at, "include"), "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(rocm, "include"), "-I" + sysconfig.get_paths()["include"], src, "-o", out, "-L" + HERE, "-l:libagarcl_hip.so", "-Wl,-rpath,$ORIGIN",
+           "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+    subprocess.check_call(cmd)
+    return out
+
+
 if __name__ == "__main__":
     if "--profile" in sys.argv:
         os.makedirs(os.path.join(HERE, "..", "build_variants"), exist_ok=True)
@@ -146,5 +173,8 @@ if __name__ == "__main__":
         print(resource_table(sys.argv[sys.argv.index("--resources") + 1]), "kernels")
     elif "--pybind" in sys.argv:
         print(build_pybind(True))
+    elif "--learn" in sys.argv:
+        print(build_learn_torch(True))
     else:
         print(build(force="--force" in sys.argv, verbose="-v" in sys.argv, single="--single" in sys.argv))
+        print(build_learn_torch(force="--force" in sys.argv))

@@ -25,6 +25,10 @@ IDS = ["f32", "bf16", "f16"]
 
 @pytest.fixture(scope="module")
 def learn(hip_engine_cls):
+    import os
+    from agarcl_amd import build
+    if not os.path.exists(build.learn_torch_out()):
+        build.build_learn_torch()
     from agarcl_amd import learn as module
     return module
 
@@ -528,6 +532,17 @@ def test_policy_loss_gradient_twice_and_with_other_upstreams(learn):
     p["old_log_prob"].add_(1)
     with pytest.raises(RuntimeError):
         out.loss.backward()
+
+
+def test_no_gradients_of_gradients(learn):
+    x = torch.randn(3, 2, 4, device="cuda", requires_grad=True)
+    h, _ = learn.gated_recurrence(x, torch.randn(3, 2, 4, device="cuda"))
+    with pytest.raises(RuntimeError, match="gradients of gradients"):
+        torch.autograd.grad(h.sum(), x, create_graph=True)
+    z = torch.randn(5, 3, device="cuda", requires_grad=True)
+    out = learn.policy_loss(z, torch.zeros(5, dtype=torch.int32, device="cuda"), torch.zeros(5, device="cuda"), torch.ones(5, device="cuda"))
+    with pytest.raises(RuntimeError, match="gradients of gradients"):
+        torch.autograd.grad(out.loss, z, create_graph=True)
 
 
 def test_policy_loss_gradient_against_differences(learn):

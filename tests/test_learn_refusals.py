@@ -6,8 +6,14 @@ import re
 import pytest
 import torch
 
-from agarcl_amd import _capi, learn
+from agarcl_amd import _capi, build
 from conftest import ROOT
+
+if not os.path.exists(_capi.HIP_SO):
+    build.build()
+if not os.path.exists(build.learn_torch_out()):
+    build.build_learn_torch()
+from agarcl_amd import learn  # noqa: E402
 
 f32, bf16 = torch.float32, torch.bfloat16
 z = torch.zeros
@@ -15,8 +21,6 @@ z = torch.zeros
 
 @pytest.fixture(scope="module")
 def lib():
-    from agarcl_amd import build
-    build.build()
     return _capi.hip_lib()
 
 
