@@ -28,7 +28,9 @@ struct DeviceScope {
 #define ON_DEVICE(dev) DeviceScope scope_(dev); if (scope_.err != hipSuccess) return fail(AGARCL_E_HIP, "device", hipGetErrorString(scope_.err))
 static int launched(const char *what) { const hipError_t e = hipGetLastError(); return e == hipSuccess ? AGARCL_OK : fail(AGARCL_E_HIP, what, hipGetErrorString(e)); }
 #define BY_TYPE(dt, ...) do { switch (dt) { case AGARCL_F32: { using T = float; __VA_ARGS__; break; } case AGARCL_BF16: { using T = bf16_t; __VA_ARGS__; break; } default: { using T = f16_t; __VA_ARGS__; break; } } } while (0)
-#define BY_VEC(vec, WIDE, ...) do { if ((vec) == WIDE) { constexpr int V = WIDE; __VA_ARGS__; } else { constexpr int V = 1; __VA_ARGS__; } } while (0)
+// (4 bytes of columns per thread; the columns of one thread are always one row's where the width is a multiple of their number; a single column cannot be two)
+#define BY_VEC(...) do { constexpr int W = 4 / sizeof(T); if (k < W) { constexpr int V = 1, R = 1; __VA_ARGS__; } else if (a->width % W == 0) { constexpr int V = W, R = 1; __VA_ARGS__; } \
+                         else { constexpr int V = W, R = W; __VA_ARGS__; } } while (0)
 static bool type_ok(int32_t dt) { return dt == AGARCL_F32 || dt == AGARCL_BF16 || dt == AGARCL_F16; }
 static const int64_t kMost = (int64_t)1 << 40;      // no dimension, stride or product of dimensions above this: 64-bit index arithmetic cannot overflow
 static bool sizes_ok(int64_t a, int64_t b, int64_t c) {
@@ -37,6 +39,7 @@ static bool sizes_ok(int64_t a, int64_t b, int64_t c) {
   return a <= kMost / b && a * b <= kMost / c;
 }
 static bool stride_ok(int64_t s, int64_t steps, int64_t least) { return steps <= 1 || (s >= least && s <= kMost && s <= (kMost << 10) / steps); }
+static int64_t reach(std::initializer_list<int64_t> strides, int64_t bytes) { int64_t m = 0; for (int64_t s : strides) if (s > m) m = s; return m * bytes; }      // from a step to the next, at most
 static unsigned blocks_for(int64_t threads) { const int64_t n = (threads + 255) / 256; return (unsigned)(n < 65536 ? n : 65536); }   // (the kernels go on in strides of the grid)
 
 // ---- recurrence -----------------------------------------------------------------------------------------------------------------------------
@@ -64,14 +67,18 @@ extern "C" int agarcl_recurrence(const agarcl_recurrence_args *a) {
   const hipStream_t st = (hipStream_t)a->stream;
   if (a->steps == 0) {      // (the state as it is)
     k_copy_state<<<dim3(blocks_for(k)), 256, 0, st>>>(a->state, a->last, k);
+  } else if (a->steps == 1) {
+    BY_TYPE(a->dtype, {
+      if (a->width % 4 == 0) k_recurrence_step<T, 4><<<dim3(blocks_for(k / 4)), 256, 0, st>>>((const T *)a->x, (const T *)a->gate, a->state, a->reset, (T *)a->h, a->last, a->marks, k, a->width);
+      else k_recurrence_step<T, 1><<<dim3(blocks_for(k)), 256, 0, st>>>((const T *)a->x, (const T *)a->gate, a->state, a->reset, (T *)a->h, a->last, a->marks, k, a->width);
+    });
   } else BY_TYPE(a->dtype, {
-    constexpr int wide = 4;
-    const ScanPlan p = scan_plan(a->steps, k, wide);
-    BY_VEC(p.vec, wide, {
-    RecurrenceOp<T, V> op;
-    op.x = (const T *)a->x; op.gate = (const T *)a->gate; op.xs = a->x_stride; op.gs = a->gate_stride; op.reset = a->reset; op.rs = a->reset_stride; op.h = (T *)a->h;
-    op.marks = a->marks; op.steps = a->steps; op.columns = k; op.width = a->width;
-    scan_launch<RecurrenceOp<T, V>, V>(op, p.sh, a->state, a->last, a->work, st);
+    BY_VEC({
+      using Op = RecurrenceOp<T, V, R>;
+      Op op;
+      op.x = {(uintptr_t)a->x, a->x_stride}; op.gate = {(uintptr_t)a->gate, a->gate_stride}; op.resets.reset = a->reset; op.resets.rs = a->reset_stride;
+      op.resets.width = a->width; op.h = {(uintptr_t)a->h, k}; op.marks = {(uintptr_t)a->marks, k}; op.steps = a->steps;
+      scan_launch<Op, V>(op, scan_shape(a->steps, k, V, reach({a->x_stride, a->gate_stride, k}, sizeof(T))), a->state, a->last, a->work, st);
     });
   });
   return launched("recurrence");
@@ -88,13 +95,13 @@ extern "C" int agarcl_recurrence_grad(const agarcl_recurrence_args *a) {
   if (a->steps == 0) {
     k_copy_state<<<dim3(blocks_for(k)), 256, 0, st>>>(a->dlast, a->dstate, k);
   } else BY_TYPE(a->dtype, {
-    constexpr int wide = sizeof(T) == 4 ? 2 : 4;
-    const ScanPlan p = scan_plan(a->steps, k, wide);
-    BY_VEC(p.vec, wide, {
-    RecurrenceGradOp<T, V> op;
-    op.x = (const T *)a->x; op.gate = (const T *)a->gate; op.dh = (const T *)a->dh; op.xs = a->x_stride; op.gs = a->gate_stride; op.ds = a->dh_stride; op.reset = a->reset;
-    op.rs = a->reset_stride; op.marks = a->marks; op.dx = (T *)a->dx; op.dgate = (T *)a->dgate; op.steps = a->steps; op.columns = k; op.width = a->width;
-    scan_launch<RecurrenceGradOp<T, V>, V>(op, p.sh, a->dlast, a->dstate, a->work, st);
+    BY_VEC({
+      using Op = RecurrenceGradOp<T, V, R>;
+      Op op;
+      op.x = {(uintptr_t)a->x, a->x_stride}; op.gate = {(uintptr_t)a->gate, a->gate_stride}; op.dh = {(uintptr_t)a->dh, a->dh_stride};
+      op.resets.reset = a->reset; op.resets.rs = a->reset_stride; op.resets.width = a->width; op.marks = {(uintptr_t)a->marks, k}; op.dx = {(uintptr_t)a->dx, k};
+      op.dgate = {(uintptr_t)a->dgate, k}; op.steps = a->steps;
+      scan_launch<Op, V>(op, scan_shape(a->steps, k, V, reach({a->x_stride, a->gate_stride, a->dh ? a->dh_stride : 0, k}, sizeof(T))), a->dlast, a->dstate, a->work, st);
     });
   });
   return launched("recurrence gradient");
@@ -117,14 +124,13 @@ extern "C" int agarcl_advantages(const agarcl_advantages_args *a) {
   if (agarcl_advantages_work(a->steps, a->rows) > 0 && !a->work) return fail(AGARCL_E_INVALID, "work");
   ON_DEVICE(a->device);
   const hipStream_t st = (hipStream_t)a->stream;
-  const ScanPlan p = scan_plan(a->steps, a->rows, 4);
-  BY_TYPE(a->dtype, BY_VEC(p.vec, 4, {
-    AdvantageOp<T, V> op;
-    op.reward = a->reward; op.value = (const T *)a->value; op.next_value = (const T *)a->next_value; op.terminated = a->terminated; op.truncated = a->truncated;
-    op.final_value = (const T *)a->final_value; op.rs = a->reward_stride; op.vs = a->value_stride; op.es = a->terminated_stride; op.us = a->truncated_stride; op.fs = a->final_stride;
-    op.gamma = a->gamma; op.gl = a->gamma * a->lambda; op.advantage = a->advantage; op.returns = a->returns; op.steps = a->steps; op.columns = a->rows;
-    scan_launch<AdvantageOp<T, V>, V>(op, p.sh, nullptr, nullptr, a->work, st);
-  }));
+  BY_TYPE(a->dtype, {
+    AdvantageOp<T, 1> op;
+    op.reward = {(uintptr_t)a->reward, a->reward_stride}; op.value = {(uintptr_t)a->value, a->value_stride}; op.final_value = {(uintptr_t)a->final_value, a->final_stride};
+    op.next_value = (const T *)a->next_value; op.terminated = a->terminated; op.truncated = a->truncated; op.es = a->terminated_stride; op.us = a->truncated_stride;
+    op.gamma = a->gamma; op.gl = a->gamma * a->lambda; op.advantage = {(uintptr_t)a->advantage, a->rows}; op.returns = {(uintptr_t)a->returns, a->rows}; op.steps = a->steps;
+    scan_launch<AdvantageOp<T, 1>, 1>(op, scan_shape(a->steps, a->rows, 1, reach({a->reward_stride, a->value_stride, a->final_value ? a->final_stride : 0, a->rows}, 4)), nullptr, nullptr, a->work, st);
+  });
   return launched("advantages");
 }
 
@@ -177,7 +183,7 @@ extern "C" int agarcl_policy_loss(const agarcl_policy_loss_args *a) {
     if (const int rc = launched("policy loss")) return rc;
   }
   if (a->want_stats) {
-    k_loss_stats<<<dim3(1), 1024, 0, st>>>(*a, (int)grid);
+    k_loss_stats<<<dim3(1), 512, 0, st>>>(*a, (int)grid);
     if (const int rc = launched("policy loss: sums")) return rc;
   }
   return AGARCL_OK;

@@ -16,50 +16,83 @@ template <class T> __device__ __forceinline__ float log_std_at(const void *p, in
 __global__ __launch_bounds__(256) void k_weight_sum(const float *__restrict__ w, int64_t rows, double *__restrict__ out) {
   __shared__ double part[4];
   double s = 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows; i += (int64_t)gridDim.x * 256) s += (double)w[i];
+  int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  for (; i + 4 <= rows; i += (int64_t)gridDim.x * 1024) {
+    Raw<float, 4> r; load_raw<float, 4>(r, w + i, 4);
+    s += ((double)r[0] + (double)r[1]) + ((double)r[2] + (double)r[3]);
+  }
+  for (; i < rows; ++i) s += (double)w[i];      // (one thread's: the others' i is beyond rows, or their four were whole)
   s = wave_sum(s);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
   __syncthreads();
   if (threadIdx.x == 0) out[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
-// bit k: kind k of these VE may be chosen
-template <int VE> __device__ __forceinline__ uint32_t load_allowed(const uint8_t *p, int nv) {
-  uint32_t bits = 0;
-  if (VE == 8 && nv == 8) {
-    struct __attribute__((packed)) Eight { uint32_t w[2]; };
-    const Eight e = *(const Eight *)p;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) bits |= (e.w[k / 4] >> (8 * (k % 4))) & 255u ? 1u << k : 0u;
-  } else {
-#pragma unroll
-    for (int k = 0; k < VE; ++k) if (k < nv) bits |= p[k] ? 1u << k : 0u;
-  }
-  return bits;
-}
-
-// VE neighbouring logits of a row: what is not allowed, or not there, as -inf
+// VE neighbouring logits of a row, still as they were loaded; what is not allowed, or not there, is made -inf in place, once, so that nothing after it
+// needs to know
 template <class T, int VE> struct Kinds {
-  Raw<T, VE> raw; uint32_t ok;
+  Raw<T, VE> raw; uint32_t ok[(VE + 3) / 4];
   __device__ __forceinline__ void load(const T *z, const uint8_t *allowed, int nv) {
     load_raw<T, VE>(raw, z, nv);
-    ok = allowed ? load_allowed<VE>(allowed, nv) : (1u << nv) - 1u;
+    if (allowed) {
+      struct __attribute__((packed)) Bytes { uint8_t b[VE]; };
+      if (nv == VE) { ok[(VE - 1) / 4] = 0; __builtin_memcpy(ok, (const Bytes *)allowed, VE); }
+      else {
+#pragma unroll
+        for (int k = 0; k < VE; k += 4) {
+          ok[k / 4] = 0;
+#pragma unroll
+          for (int i = 0; i < 4 && k + i < VE; ++i) if (k + i < nv) ok[k / 4] |= (uint32_t)allowed[k + i] << (8 * i);
+        }
+      }
+    }
   }
-  __device__ __forceinline__ float operator[](int k) const { return (ok >> k) & 1 ? raw[k] : -INFINITY; }
+  __device__ __forceinline__ void mask(bool flags, int nv) {
+    if (flags) {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) if constexpr (sizeof(T) == 4) {
+        if (!(ok[k / 4] >> (8 * (k % 4)) & 255u)) raw.w[k] = 0xff800000u;
+      }
+      if constexpr (sizeof(T) == 2) {      // two at a time: 0 / nonzero bytes to 0 / 0xffff halves
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        const uint32_t none = std::is_same<T, bf16_t>::value ? 0xff80ff80u : 0xfc00fc00u;
+#pragma unroll
+        for (int k = 0; k < (VE + 1) / 2; ++k) {
+          const uint32_t pair = __builtin_amdgcn_perm(0u, ok[k / 2], k & 1 ? 0x0c030c02u : 0x0c010c00u);
+          u16x2 h = __builtin_bit_cast(u16x2, pair);
+          h = (u16x2)(0) - __builtin_elementwise_min(h, (u16x2)(1));
+          const uint32_t m = __builtin_bit_cast(uint32_t, h);
+          raw.w[k] = (raw.w[k] & m) | (none & ~m);
+        }
+      }
+    }
+    if (nv < VE) {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) if (k >= nv) {
+        if constexpr (sizeof(T) == 4) raw.w[k] = 0xff800000u;
+        else { const uint32_t none = std::is_same<T, bf16_t>::value ? 0xff80u : 0xfc00u; raw.w[k / 2] = k & 1 ? (raw.w[k / 2] & 0xffffu) | none << 16 : (raw.w[k / 2] & 0xffff0000u) | none; }
+      }
+    }
+  }
+  __device__ __forceinline__ float operator[](int k) const { return raw[k]; }
 };
 
-// what a row's kinds come to, relative to the maximum m
+// what a row's kinds come to, relative to the maximum m: s = sum of e^(z - m), u = sum of e^(z - m) (z - m)
 struct RowSums { float m, s, u; };
-__device__ __forceinline__ float exp_below(float z, float m) { return z == -INFINITY ? 0.f : __expf(z - m); }
-__device__ __forceinline__ void sums_add(RowSums &r, float z, float e) { r.s += e; if (e > 0.f) r.u += e * (z - r.m); }
+// z - m, and nothing so low that the product with e^(z - m) = 0 would not be 0
+// (the maximum that passes a NaN on: a NaN among the logits is to be seen in the loss)
+__device__ __forceinline__ float below(float z, float m) { return __builtin_elementwise_maximum(z - m, -200.f); }
+// the reference point of a row: its maximum, or anything finite where nothing is allowed
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+__device__ __forceinline__ void sums_add(RowSums &r, float z) { const float d = below(z, r.m), e = __expf(d); r.s += e; r.u = fmaf(e, d, r.u); }
 // r's sums relative to another maximum
 __device__ __forceinline__ void sums_shift(RowSums &r, float m) {
-  if (r.s > 0.f && m != r.m) { const float d = r.m - m, k = __expf(d); r.u = k * (r.u + r.s * d); r.s *= k; }
+  if (r.s > 0.f && m != r.m) { const float d = below(r.m, m), k = __expf(d); r.u = k * fmaf(r.s, d, r.u); r.s *= k; }
   r.m = m;
 }
 
 // everything of a row that is not per kind
-struct LossRow { bool counts; int32_t kind; float share, g, log_s, hcat, dev[2], istd[2]; };
+struct LossRow { bool counts; int32_t kind; float sg, c0, c1; };      // dlogit[j] = p[j] (c1 (z[j] - m) + c0) + (j == kind ? sg : 0)
 struct LossTotals { float inv; bool shared_std; };
 
 template <class T> __device__ __forceinline__ LossRow loss_row(const agarcl_policy_loss_args &a, const LossTotals &t, int64_t row, const RowSums &r, const T *z, const uint8_t *ok,
@@ -70,46 +103,46 @@ template <class T> __device__ __forceinline__ LossRow loss_row(const agarcl_poli
   o.counts = w != 0.f && kind >= 0 && kind < a.kinds;
   float za = 0.f;
   if (o.counts) { za = to_f(z[kind]); o.counts = za != -INFINITY && (!ok || ok[kind]); }
-  o.log_s = logf(r.s); o.hcat = o.log_s - r.u / r.s;
-  float lp = za - r.m - o.log_s, ent = o.hcat;
-#pragma unroll
-  for (int d = 0; d < 2; ++d) o.dev[d] = o.istd[d] = 0.f;
+  const float log_s = logf(r.s), rs = 1.f / r.s, hcat = log_s - r.u * rs;
+  float lp = za - r.m - log_s, ent = hcat;
+  float dev[2] = {0.f, 0.f}, istd[2] = {0.f, 0.f};
   if (a.mean) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
       const float ls = log_std_at<T>(a.log_std, a.log_std_per_row, row, d);
-      o.istd[d] = expf(-ls);
-      o.dev[d] = (a.move[2 * row + d] - to_f(((const T *)a.mean)[2 * row + d])) * o.istd[d];
-      lp -= 0.5f * o.dev[d] * o.dev[d] + ls + kHalfLog2Pi;
+      istd[d] = expf(-ls);
+      dev[d] = (a.move[2 * row + d] - to_f(((const T *)a.mean)[2 * row + d])) * istd[d];
+      lp -= 0.5f * dev[d] * dev[d] + ls + kHalfLog2Pi;
       ent += ls + kHalfLog2PiE;
     }
   }
   const float ratio = expf(lp - old);
-  const float low = A == 0.f ? 0.f : fminf(ratio * A, fminf(fmaxf(ratio, 1.f - a.clip_low), 1.f + a.clip_high) * A);
   const bool clipped = A >= 0.f ? ratio > 1.f + a.clip_high : ratio < 1.f - a.clip_low;
-  const float back = ref - lp, eb = expm1f(back), kl = eb - back;      // (expm1: near 0 the KL term is the difference of near numbers)
-  o.g = clipped || A == 0.f ? 0.f : -A * ratio;
-  if (a.kl_coef != 0.f) o.g -= a.kl_coef * eb;
-  o.share = w * t.inv;
+  const float back = ref - lp, eb = expm1f(back);      // (expm1: near 0 the KL term is the difference of near numbers)
+  float g = clipped || A == 0.f ? 0.f : -A * ratio;
+  if (a.kl_coef != 0.f) g -= a.kl_coef * eb;
+  const float share = w * t.inv, ce = a.entropy_coef;
+  o.sg = share * g; o.c1 = share * ce * rs; o.c0 = (ce != 0.f ? share * ce * (hcat - log_s) - o.sg : -o.sg) * rs;
   if (leader) {
+    const float low = A == 0.f ? 0.f : fminf(ratio * A, fminf(fmaxf(ratio, 1.f - a.clip_low), 1.f + a.clip_high) * A);
     acc[0] += (double)w;
     if (o.counts) {
-      acc[1] += (double)w * low; acc[2] += (double)w * kl; acc[3] += (double)w * ent; acc[4] += clipped ? (double)w : 0.;
+      acc[1] += (double)w * low; acc[2] += (double)w * (eb - back); acc[3] += (double)w * ent; acc[4] += clipped ? (double)w : 0.;
       if (t.shared_std) {
 #pragma unroll
-        for (int d = 0; d < 2; ++d) acc[5 + d] += (double)w * (o.g * (o.dev[d] * o.dev[d] - 1.f) - a.entropy_coef);
+        for (int d = 0; d < 2; ++d) acc[5 + d] += (double)w * (g * (dev[d] * dev[d] - 1.f) - ce);
       }
     }
     if (a.dmean) {
       float v[2];
 #pragma unroll
-      for (int d = 0; d < 2; ++d) v[d] = o.counts ? o.share * o.g * o.dev[d] * o.istd[d] : 0.f;
+      for (int d = 0; d < 2; ++d) v[d] = o.counts ? o.sg * dev[d] * istd[d] : 0.f;
       store_pack<T, 2>((T *)a.dmean + 2 * row, v, 2);
     }
     if (a.dlog_std && a.log_std_per_row) {
       float v[2];
 #pragma unroll
-      for (int d = 0; d < 2; ++d) v[d] = o.counts ? o.share * (o.g * (o.dev[d] * o.dev[d] - 1.f) - a.entropy_coef) : 0.f;
+      for (int d = 0; d < 2; ++d) v[d] = o.counts ? o.sg * (dev[d] * dev[d] - 1.f) - share * ce : 0.f;
       store_pack<T, 2>((T *)a.dlog_std + 2 * row, v, 2);
     }
   }
@@ -118,16 +151,20 @@ template <class T> __device__ __forceinline__ LossRow loss_row(const agarcl_poli
 
 // the gradient of kinds j0 ... of a row.  The probabilities are worked out once more: holding 8 of them for every 4 registers of logits would cost more
 // (registers, and with them wavefronts) than a second exp
-template <class T, int VE> __device__ __forceinline__ void loss_kinds(const agarcl_policy_loss_args &a, const LossRow &o, const RowSums &r, int64_t row, int64_t j0, int nv, Kinds<T, VE> &z) {
-  const float rs = 1.f / r.s;
+template <class T, int VE> __device__ __forceinline__ void loss_kinds(const agarcl_policy_loss_args &a, const LossRow &o, float m, int64_t row, int64_t j0, int nv, Kinds<T, VE> &z) {
   z.raw.anew();
   float v[VE];
+  if (o.counts) {
 #pragma unroll
-  for (int k = 0; k < VE; ++k) {
-    const float p = exp_below(z[k], r.m) * rs;
-    float d = o.g * ((j0 + k == o.kind ? 1.f : 0.f) - p);
-    if (a.entropy_coef != 0.f && p > 0.f) d += a.entropy_coef * p * (z[k] - r.m - o.log_s + o.hcat);
-    v[k] = o.counts && (z.ok >> k) & 1 ? o.share * d : 0.f;
+    for (int k = 0; k < VE; ++k) { const float d = below(z[k], m); v[k] = __expf(d) * fmaf(o.c1, d, o.c0); }
+    const int64_t at = o.kind - j0;
+    if (at >= 0 && at < VE) {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) v[k] += k == (int)at ? o.sg : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < VE; ++k) v[k] = 0.f;
   }
   store_pack<T, VE>((T *)a.dlogits + row * a.kinds + j0, v, nv);
 }
@@ -169,7 +206,7 @@ __device__ __forceinline__ void loss_end(const agarcl_policy_loss_args &a, doubl
   if (threadIdx.x < 7) {
     double s = 0;
     for (int i = 0; i < (int)blockDim.x / 64; ++i) s += lds[8 * i + threadIdx.x];
-    a.work[8 * blockIdx.x + threadIdx.x] = s;
+    a.work[threadIdx.x * kLossBlocks + blockIdx.x] = s;
   }
 }
 
@@ -183,17 +220,58 @@ __global__ __launch_bounds__(256) void k_loss_thread(const agarcl_policy_loss_ar
   for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) {
     const T *zp = (const T *)a.logits + row * a.logits_stride;
     const uint8_t *ok = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-    Kinds<T, V> z; z.load(zp, ok, V);
+    Kinds<T, V> z; z.load(zp, ok, V); z.mask(ok, V);
     RowSums r = {-INFINITY, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < V; ++k) r.m = fmaxf(r.m, z[k]);
+    r.m = finite_max(r.m);
 #pragma unroll
-    for (int k = 0; k < V; ++k) sums_add(r, z[k], exp_below(z[k], r.m));
+    for (int k = 0; k < V; ++k) sums_add(r, z[k]);
     const LossRow o = loss_row<T>(a, t, row, r, zp, ok, true, acc);
-    if (a.dlogits) loss_kinds<T, V>(a, o, r, row, 0, V, z);
+    if (a.dlogits) loss_kinds<T, V>(a, o, r.m, row, 0, V, z);
   }
   loss_end(a, acc, lds);
 }
+
+// a thread's CHUNKS x 8 kinds of a row, chunk c at j0 + c x stride
+template <class T, int CHUNKS> struct Share {
+  Kinds<T, 8> z[CHUNKS]; int nv[CHUNKS];
+  __device__ __forceinline__ void load(const T *zp, const uint8_t *ok, int64_t j0, int64_t stride, int64_t kinds, bool on) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int64_t j = j0 + c * stride, left = kinds - j;
+      nv[c] = on ? (left < 0 ? 0 : left < 8 ? (int)left : 8) : 0;
+      z[c].load(zp + j, ok ? ok + j : nullptr, nv[c]);
+    }
+  }
+  __device__ __forceinline__ float top(bool flags) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      z[c].mask(flags, nv[c]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, z[c][k]);
+      __builtin_amdgcn_sched_barrier(0);      // (chunk after chunk: all at once would take the registers of a second wavefront)
+    }
+    return m;
+  }
+  __device__ __forceinline__ void sum(RowSums &r) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      z[c].raw.anew();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sums_add(r, z[c][k]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  __device__ __forceinline__ void gradient(const agarcl_policy_loss_args &a, const LossRow &o, float m, int64_t row, int64_t j0, int64_t stride) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      if (nv[c] > 0) loss_kinds<T, 8>(a, o, m, row, j0 + c * stride, nv[c], z[c]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
 
 // 8 << g_log (x CHUNKS) kinds, a group of 1 << g_log lanes per row
 template <class T, int CHUNKS>
@@ -208,33 +286,15 @@ __global__ __launch_bounds__(256) void k_loss_lanes(const agarcl_policy_loss_arg
     const bool on = row < a.rows;
     const T *zp = (const T *)a.logits + (on ? row : 0) * a.logits_stride;
     const uint8_t *ok = a.allowed ? a.allowed + (on ? row : 0) * a.allowed_stride : nullptr;
-    Kinds<T, 8> z[CHUNKS]; int nv[CHUNKS];
-    RowSums r = {-INFINITY, 0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-      const int64_t j0 = (int64_t)(c * g + lane) * 8, left = a.kinds - j0;
-      nv[c] = on ? (left < 0 ? 0 : left < 8 ? (int)left : 8) : 0;
-      z[c].load(zp + j0, ok ? ok + j0 : nullptr, nv[c]);
-    }
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) r.m = fmaxf(r.m, z[c][k]);
-    }
+    Share<T, CHUNKS> z; z.load(zp, ok, lane * 8, g * 8, a.kinds, on);
+    RowSums r = {z.top(ok), 0.f, 0.f};
     for (int d = 1; d < g; d <<= 1) r.m = fmaxf(r.m, __shfl_xor(r.m, d));
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-      z[c].raw.anew();
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sums_add(r, z[c][k], exp_below(z[c][k], r.m));
-    }
+    r.m = finite_max(r.m);
+    z.sum(r);
     for (int d = 1; d < g; d <<= 1) { r.s += __shfl_xor(r.s, d); r.u += __shfl_xor(r.u, d); }
     if (!on) continue;      // (a whole group, behind the last of the shuffles of this turn)
     const LossRow o = loss_row<T>(a, t, row, r, zp, ok, lane == 0, acc);
-    if (a.dlogits) {
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) loss_kinds<T, 8>(a, o, r, row, (int64_t)(c * g + lane) * 8, nv[c], z[c]);
-    }
+    if (a.dlogits) z.gradient(a, o, r.m, row, lane * 8, g * 8);
   }
   loss_end(a, acc, lds);
 }
@@ -253,6 +313,7 @@ template <int NT> __device__ __forceinline__ RowSums join_waves(const RowSums &m
     sums_shift(w, all.m);
     all.s += w.s; all.u += w.u;
   }
+  all.m = finite_max(all.m);
   return all;
 }
 
@@ -268,43 +329,29 @@ __global__ __launch_bounds__(NT) void k_loss_block(const agarcl_policy_loss_args
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
     const T *zp = (const T *)a.logits + row * a.logits_stride;
     const uint8_t *ok = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-    RowSums r = {-INFINITY, 0.f, 0.f};
     if constexpr (CHUNKS > 0) {
-      Kinds<T, 8> z[CHUNKS]; int nv[CHUNKS];
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const int64_t j0 = (int64_t)(c * NT + threadIdx.x) * 8, left = a.kinds - j0;
-        nv[c] = left < 0 ? 0 : left < 8 ? (int)left : 8;
-        z[c].load(zp + j0, ok ? ok + j0 : nullptr, nv[c]);
-      }
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) r.m = fmaxf(r.m, z[c][k]);
-      }
-      r.m = wave_max(r.m);
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        z[c].raw.anew();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sums_add(r, z[c][k], exp_below(z[c][k], r.m));
-      }
+      Share<T, CHUNKS> z; z.load(zp, ok, threadIdx.x * 8, NT * 8, a.kinds, true);
+      const float top = wave_max(z.top(ok));
+      RowSums r = {finite_max(top), 0.f, 0.f};
+      z.sum(r);
       r.s = wave_sum(r.s); r.u = wave_sum(r.u);
+      r.m = top;
       const RowSums all = join_waves<NT>(r, wl, parity);
       const LossRow o = loss_row<T>(a, t, row, all, zp, ok, threadIdx.x == 0, acc);
-      if (a.dlogits) {
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) loss_kinds<T, 8>(a, o, all, row, (int64_t)(c * NT + threadIdx.x) * 8, nv[c], z[c]);
-      }
+      if (a.dlogits) z.gradient(a, o, all.m, row, threadIdx.x * 8, NT * 8);
     } else {
+      RowSums r = {-INFINITY, 0.f, 0.f};
       for (int64_t j0 = (int64_t)threadIdx.x * 8; j0 < a.kinds; j0 += NT * 8) {
-        Kinds<T, 8> z; z.load(zp + j0, ok ? ok + j0 : nullptr, a.kinds - j0 < 8 ? (int)(a.kinds - j0) : 8);
+        const int nv = a.kinds - j0 < 8 ? (int)(a.kinds - j0) : 8;
+        Kinds<T, 8> z; z.load(zp + j0, ok ? ok + j0 : nullptr, nv); z.mask(ok, nv);
         float m = r.m;
 #pragma unroll
         for (int k = 0; k < 8; ++k) m = fmaxf(m, z[k]);
         sums_shift(r, m);
+        RowSums c = {finite_max(m), 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sums_add(r, z[k], exp_below(z[k], m));
+        for (int k = 0; k < 8; ++k) sums_add(c, z[k]);
+        r.s += c.s; r.u += c.u;
       }
       sums_shift(r, wave_max(r.m));
       r.s = wave_sum(r.s); r.u = wave_sum(r.u);
@@ -313,8 +360,8 @@ __global__ __launch_bounds__(NT) void k_loss_block(const agarcl_policy_loss_args
       if (a.dlogits) {
         for (int64_t j0 = (int64_t)threadIdx.x * 8; j0 < a.kinds; j0 += NT * 8) {
           const int nv = a.kinds - j0 < 8 ? (int)(a.kinds - j0) : 8;
-          Kinds<T, 8> z; z.load(zp + j0, ok ? ok + j0 : nullptr, nv);
-          loss_kinds<T, 8>(a, o, all, row, j0, nv, z);
+          Kinds<T, 8> z; z.load(zp + j0, ok ? ok + j0 : nullptr, nv); z.mask(ok, nv);
+          loss_kinds<T, 8>(a, o, all.m, row, j0, nv, z);
         }
       }
     }
@@ -322,22 +369,26 @@ __global__ __launch_bounds__(NT) void k_loss_block(const agarcl_policy_loss_args
   loss_end(a, acc, lds);
 }
 
-// the workgroups' sums in a fixed order: the same inputs give the same bits
-__global__ __launch_bounds__(1024) void k_loss_stats(const agarcl_policy_loss_args a, int blocks) {
-  __shared__ double part[16][8];
+// the workgroups' sums in a fixed order: the same inputs give the same bits.  One wavefront per sum, so that its loads are all under way at once (a wavefront that
+// took all seven in turn needed 6.7 us for 2048 workgroups)
+__global__ __launch_bounds__(512) void k_loss_stats(const agarcl_policy_loss_args a, int blocks) {
+  __shared__ double sums[8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double acc[7] = {0, 0, 0, 0, 0, 0, 0};
-  for (int b = threadIdx.x; b < blocks; b += 1024) for (int i = 0; i < 7; ++i) acc[i] += a.work[8 * b + i];
-  for (int i = 0; i < 7; ++i) { acc[i] = wave_sum(acc[i]); if (lane == 0) part[wave][i] = acc[i]; }
+  if (wave < 7) {
+    double s = 0;
+#pragma unroll 8
+    for (int b = lane; b < blocks; b += 64) s += a.work[wave * kLossBlocks + b];
+    s = wave_sum(s);
+    if (lane == 0) sums[wave] = s;
+  }
   __syncthreads();
   if (threadIdx.x) return;
-  for (int i = 0; i < 7; ++i) { acc[i] = 0; for (int w = 0; w < 16; ++w) acc[i] += part[w][i]; }
-  const double inv = acc[0] != 0 ? 1. / acc[0] : 0., by = a.mean_over_weight ? inv : 1.;
-  const double kl = a.kl_coef != 0.f ? (double)a.kl_coef * acc[2] : 0., ent = a.entropy_coef != 0.f ? (double)a.entropy_coef * acc[3] : 0.;
-  a.loss[0] = (float)((kl - acc[1] - ent) * by);
-  for (int i = 1; i < 5; ++i) a.stats[i - 1] = (float)(acc[i] * inv);
-  a.stats[4] = (float)acc[0]; a.stats[5] = a.stats[6] = a.stats[7] = 0.f;
-  if (a.dlog_std && !a.log_std_per_row) for (int d = 0; d < 2; ++d) ((float *)a.dlog_std)[d] = (float)(acc[5 + d] * by);
+  const double inv = sums[0] != 0 ? 1. / sums[0] : 0., by = a.mean_over_weight ? inv : 1.;
+  const double kl = a.kl_coef != 0.f ? (double)a.kl_coef * sums[2] : 0., ent = a.entropy_coef != 0.f ? (double)a.entropy_coef * sums[3] : 0.;
+  a.loss[0] = (float)((kl - sums[1] - ent) * by);
+  for (int i = 1; i < 5; ++i) a.stats[i - 1] = (float)(sums[i] * inv);
+  a.stats[4] = (float)sums[0]; a.stats[5] = a.stats[6] = a.stats[7] = 0.f;
+  if (a.dlog_std && !a.log_std_per_row) for (int d = 0; d < 2; ++d) ((float *)a.dlog_std)[d] = (float)(sums[5 + d] * by);
 }
 
 // how many kinds call for which kernel; the workgroups a launch needs
@@ -376,7 +427,7 @@ struct Pick { RowSums r; float best; int at; };
 __device__ __forceinline__ void pick_join(Pick &p, float best, int at) { if (at != NONE && (p.at == NONE || best > p.best || (best == p.best && at < p.at))) { p.best = best; p.at = at; } }
 
 template <class T, int VE> __device__ __forceinline__ void pick_kinds(Pick &p, const T *z, const uint8_t *ok, const float *gum, int64_t j0, int nv) {
-  Kinds<T, VE> k; k.load(z + j0, ok ? ok + j0 : nullptr, nv);
+  Kinds<T, VE> k; k.load(z + j0, ok ? ok + j0 : nullptr, nv); k.mask(ok, nv);
   Raw<float, VE> gu;
   if (gum) load_raw<float, VE>(gu, gum + j0, nv);
   float m = p.r.m;
@@ -387,7 +438,7 @@ template <class T, int VE> __device__ __forceinline__ void pick_kinds(Pick &p, c
   for (int i = 0; i < VE; ++i) {
     const float v = k[i];
     if (v == -INFINITY) continue;
-    p.r.s += __expf(v - m);
+    p.r.s += __expf(below(v, m));
     const float score = gum ? v + gu[i] : v;
     if (p.at == NONE || score > p.best) { p.best = score; p.at = (int)(j0 + i); }      // (indices rise within a thread: the first of equals stays)
   }

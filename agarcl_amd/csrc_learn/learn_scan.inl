@@ -1,18 +1,27 @@
 // learn_scan.inl -- linear recurrences y[t] = a[t] y[t-1] + b[t] over the steps of a rollout, for many columns at once.
 //
-// A segment is 8 steps (AGARCL_MARK_STEPS).  One thread owns a segment of VEC neighbouring columns: it loads the segment once into registers, works out the
-// segment's own map y -> P y + B, and -- when it knows the y that enters -- goes through the steps again from registers and writes.  A workgroup is CL column
-// lanes x TL = 256 / CL time lanes and takes TL segments in a row at once: the maps are joined over the time lanes of a wavefront by shuffles and over the
-// wavefronts through LDS, with one barrier per TL segments.  Column lanes are the fast index of a wavefront, so its loads are runs of CL x VEC elements.
-// Where there are too few columns to fill the chip the steps are cut into chunks as well: a first launch leaves every chunk's map, the second starts each chunk
-// from the maps in front of it.
+// A segment is 8 steps (AGARCL_MARK_STEPS).  One thread owns a segment of VEC neighbouring columns: it loads the segment into registers and works out, step by
+// step, y[i] = P[i] y + B[i] over the y that enters -- before it knows that y.  A workgroup is CL column lanes x TL = 256 / CL time lanes and takes TL segments in
+// a row at once: the segments' maps are joined over the time lanes of a wavefront by shuffles and over the wavefronts through LDS, with one barrier per TL
+// segments, and then every step is one multiplication and addition away.  The next segment's loads are under way meanwhile.  Column lanes are the fast index
+// of a wavefront, so its loads are runs of CL x VEC elements.  Where there are too few columns to fill the chip the steps are cut into chunks as well: a
+// first launch leaves every chunk's map, the second starts each chunk from the maps in front of it.
 //
 // A map's P is 0 exactly where a step of it drops what came before (a reset, the end of an episode): joining looks at P and never multiplies what was
 // dropped, so infinities and NaN do not pass.  A product of gates is kept from underflowing to 0 (times 1e-38 is nothing in 32 bits all the same).
+#define GLOBAL __attribute__((address_space(1)))
+
 // VEC neighbouring elements as they were loaded: 16-bit ones stay two to a register
 template <class T, int VEC> struct Raw {
   uint32_t w[(VEC * sizeof(T) + 3) / 4];
   __device__ __forceinline__ float operator[](int j) const;
+  __device__ __forceinline__ void all(T v) {
+    uint32_t b;
+    if constexpr (sizeof(T) == 4) b = __builtin_bit_cast(uint32_t, v);
+    else b = __builtin_bit_cast(uint16_t, v) * 0x10001u;
+#pragma unroll
+    for (auto &r : w) r = b;
+  }
   // a later use takes the registers from here on: keeps the compiler from holding what it derived from them (a gate's sigmoids) in twice as many
   __device__ __forceinline__ void anew() {
 #pragma unroll
@@ -27,34 +36,41 @@ template <class T, int VEC> __device__ __forceinline__ float Raw<T, VEC>::operat
 // (aligned as an element is, no more: the hardware takes wide loads at any address)
 template <class T, int VEC> struct __attribute__((packed, aligned(alignof(T)))) Pack { T v[VEC]; };
 
+template <class T, int VEC> __device__ __forceinline__ void load_raw(Raw<T, VEC> &out, const T *p) {
+  out.w[(VEC * sizeof(T) - 1) / 4] = 0;
+  __builtin_memcpy(out.w, (const Pack<T, VEC> *)p, VEC * sizeof(T));
+}
+// the first nv of them; the others 0
 template <class T, int VEC> __device__ __forceinline__ void load_raw(Raw<T, VEC> &out, const T *p, int nv) {
-  if constexpr (VEC * sizeof(T) < 4) { out.w[0] = nv ? (uint32_t)*(const uint16_t *)p : 0u; }
+  if (nv == VEC) load_raw<T, VEC>(out, p);
   else {
-    if (nv == VEC) __builtin_memcpy(out.w, (const Pack<T, VEC> *)p, VEC * sizeof(T));
-    else {
 #pragma unroll
-      for (int k = 0; k < (int)(VEC * sizeof(T) / 4); ++k) {
-        if constexpr (sizeof(T) == 4) out.w[k] = k < nv ? ((const uint32_t *)p)[k] : 0u;
-        else out.w[k] = (2 * k < nv ? (uint32_t)((const uint16_t *)p)[2 * k] : 0u) | (2 * k + 1 < nv ? (uint32_t)((const uint16_t *)p)[2 * k + 1] << 16 : 0u);
-      }
+    for (int k = 0; k < (int)(VEC * sizeof(T) + 3) / 4; ++k) {
+      if constexpr (sizeof(T) == 4) out.w[k] = k < nv ? ((const uint32_t *)p)[k] : 0u;
+      else out.w[k] = (2 * k < nv ? (uint32_t)((const uint16_t *)p)[2 * k] : 0u) | (2 * k + 1 < nv ? (uint32_t)((const uint16_t *)p)[2 * k + 1] << 16 : 0u);
     }
   }
 }
-template <int VEC> __device__ __forceinline__ void load_floats(float (&out)[VEC], const float *p, int nv) {
-  Raw<float, VEC> r; load_raw<float, VEC>(r, p, nv);
+template <int VEC> __device__ __forceinline__ void load_floats(float (&out)[VEC], const float *p) {
+  Raw<float, VEC> r; load_raw<float, VEC>(r, p);
 #pragma unroll
   for (int j = 0; j < VEC; ++j) out[j] = r[j];
 }
-template <class T, int VEC> __device__ __forceinline__ void store_pack(T *p, const float (&in)[VEC], int nv) {
+template <class T, int VEC> __device__ __forceinline__ void store_pack(T *p, const float (&in)[VEC]) {
   Pack<T, VEC> k;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) k.v[j] = from_f<T>(in[j]);
-  if (nv == VEC) *(Pack<T, VEC> *)p = k;
+  *(Pack<T, VEC> *)p = k;
+}
+template <class T, int VEC> __device__ __forceinline__ void store_pack(T *p, const float (&in)[VEC], int nv) {
+  if (nv == VEC) store_pack<T, VEC>(p, in);
   else {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) if (j < nv) p[j] = k.v[j];
+    for (int j = 0; j < VEC; ++j) if (j < nv) p[j] = from_f<T>(in[j]);
   }
 }
+// device memory at an address that is the same for the wavefront and an offset that is the lane's: the form that loads take without vector arithmetic
+template <class T> __device__ __forceinline__ T *device_ptr(uintptr_t base, uint32_t off) { return (T *)(GLOBAL T *)((GLOBAL char *)base + off); }
 
 template <int VEC> struct Map { float P[VEC], B[VEC]; };
 __device__ __forceinline__ float map_at(float P, float B, float y) { return P == 0.f ? B : fmaf(P, y, B); }
@@ -69,8 +85,10 @@ template <int VEC> __device__ __forceinline__ void map_behind(Map<VEC> &m, const
   for (int j = 0; j < VEC; ++j) { m.B[j] = map_at(m.P[j], m.B[j], e.B[j]); m.P[j] = map_p(m.P[j], e.P[j]); }
 }
 
-// the shape of a launch: chosen on the host (scan_plan)
-struct ScanShape { int cl_log, chunks; int64_t segments, chunk_segments, columns, groups; };
+static const int SEG = AGARCL_MARK_STEPS;
+
+// the shape of a launch: chosen on the host (scan_shape)
+struct ScanShape { int cl_log, chunks; int64_t segments, chunk_segments, columns, groups, slots; };      // slots: groups, up to a multiple of 8
 
 template <int VEC> struct ScanLds { Map<VEC> total[2][256]; };   // [parity][wavefront (or pair, or all four) x column lane]
 
@@ -111,29 +129,50 @@ template <int VEC> __device__ __forceinline__ void scan_join(const ScanLane &s, 
   map_behind(before, front);
 }
 
-// Op: load(segment) -> registers, map(Map &), run(segment, float (&y)[VEC]) goes through the steps from y and writes.  Op::reverse: the last segment is first.
+// Where a thread's segment lies: step t0 of the rollout, `t` steps behind step `base`, which is the same for the workgroup; its columns are `c` behind column
+// `cbase`.  An array's address is then one scalar register pair, a step's stride away from the next step's, and a 32-bit offset of the thread's: no vector
+// arithmetic per load.  The offsets fit: see scan_shape.
+struct Place { int64_t base, cbase; uint32_t t, c; };
+template <class T> struct Rows {      // an array of steps x columns
+  uintptr_t p; int64_t stride;
+  __device__ __forceinline__ uint32_t offset(const Place &w) const { return (w.t * (uint32_t)stride + w.c) * (uint32_t)sizeof(T); }
+  __device__ __forceinline__ uintptr_t first(const Place &w) const { return p + (w.base * stride + w.cbase) * (int64_t)sizeof(T); }      // the same for the workgroup
+  __device__ __forceinline__ int64_t step() const { return stride * (int64_t)sizeof(T); }
+};
+
+// Op: load(place) -> registers; prep(Map &): what can be known without the y that enters; write(place, y).  Op::reverse: the last segment is first.
 // work: [2][chunks][columns] maps of the chunks
 template <class Op, int VEC, bool MAPS>
 __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const float *start, float *end, float *work, ScanLds<VEC> &lds) {
   const ScanLane s = scan_lane(sh.cl_log);
   int parity = 0;
   const int64_t q = blockIdx.y, first = q * sh.chunk_segments, stop = first + sh.chunk_segments < sh.segments ? first + sh.chunk_segments : sh.segments;
-  for (int64_t group = blockIdx.x; group < sh.groups; group += gridDim.x) {
-    const int64_t c0 = ((group << sh.cl_log) + s.col) * VEC;
-    const int nv = c0 >= sh.columns ? 0 : sh.columns - c0 < VEC ? (int)(sh.columns - c0) : VEC;
-    op.place(c0, nv);
+  for (int64_t b = blockIdx.x; b < sh.slots; b += gridDim.x) {
+    // neighbouring column groups share 128-byte lines where they are narrow: keep them on one XCD, behind one L2 (workgroups go to the 8 XCDs in turn)
+    const int64_t group = sh.slots >= 16 ? (b & 7) * (sh.slots >> 3) + (b >> 3) : b;
+    if (group >= sh.groups) continue;
+    const int64_t cbase = (group << sh.cl_log) * VEC;
+    int64_t c0 = cbase + s.col * VEC;
+    const bool there = c0 < sh.columns;
+    // (the last thread of a row of columns that VEC does not divide takes some of its neighbour's, too, and writes the same there)
+    if (there && c0 + VEC > sh.columns) c0 = sh.columns - VEC;
+    op.start(there ? c0 : 0);
+    // the turn that begins with segment k0 (counted in the scan's order)
+    const auto place = [&](int64_t k0) __attribute__((always_inline)) {
+      return Place{(Op::reverse ? sh.segments - s.tls - k0 : k0) * SEG, cbase, (uint32_t)(Op::reverse ? s.tls - 1 - s.tl : s.tl) * SEG, (uint32_t)(c0 - cbase)};
+    };
     float y[VEC];
     Map<VEC> run; map_clear(run);
     if (!MAPS) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) y[j] = start && j < nv ? start[c0 + j] : 0.f;
+      for (int j = 0; j < VEC; ++j) y[j] = start && there ? start[c0 + j] : 0.f;
       if (q) {      // the chunks in front: each time lane joins a part of their maps, then all of them
         const int64_t each = (q + s.tls - 1) / s.tls, lo = s.tl * each, hi = lo + each < q ? lo + each : q;
         Map<VEC> m, before, all; map_clear(m);
-        for (int64_t k = lo; k < hi; ++k) if (nv) {
+        for (int64_t c = lo; c < hi; ++c) if (there) {
           Map<VEC> t;
-          const float *p = work + k * sh.columns + c0, *b = p + sh.chunks * sh.columns;
-          load_floats<VEC>(t.P, p, nv); load_floats<VEC>(t.B, b, nv);
+          const float *p = work + c * sh.columns + c0, *b = p + sh.chunks * sh.columns;
+          load_floats<VEC>(t.P, p); load_floats<VEC>(t.B, b);
           map_behind(t, m); m = t;
         }
         scan_join(s, m, before, all, lds, parity); parity ^= 1;
@@ -141,35 +180,33 @@ __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const 
         for (int j = 0; j < VEC; ++j) y[j] = map_at(all.P[j], all.B[j], y[j]);
       }
     }
-    for (int64_t k0 = first; k0 < stop; k0 += s.tls) {
-      const int64_t k = k0 + s.tl, seg = Op::reverse ? sh.segments - 1 - k : k;
-      const bool on = k < stop && nv > 0;
-      if (on) op.load(seg);
-      float in[VEC];
+    for (int64_t k0 = first - s.tls; k0 < stop; k0 += s.tls) {      // (one turn early: it loads the first segments and does nothing else)
+      const bool turn = k0 >= first, on = turn && k0 + s.tl < stop && there;
+      Map<VEC> m;
+      map_clear(m);
+      if (on) op.prep(m);
+      if (k0 + s.tls + s.tl < stop && there) op.load(place(k0 + s.tls));      // (under way while the maps are joined and the steps written)
+      if (!turn) continue;
+      float e[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) in[j] = MAPS ? 0.f : y[j];
+      for (int j = 0; j < VEC; ++j) e[j] = MAPS ? 0.f : y[j];
       if (MAPS || s.tls > 1) {
-        Map<VEC> m, before, all;
-        map_clear(m);
-        if (on) op.map(m);
+        Map<VEC> before, all;
         scan_join(s, m, before, all, lds, parity); parity ^= 1;
         if (MAPS) { map_behind(all, run); run = all; }
         else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) { in[j] = map_at(before.P[j], before.B[j], y[j]); y[j] = map_at(all.P[j], all.B[j], y[j]); }
+          for (int j = 0; j < VEC; ++j) { e[j] = map_at(before.P[j], before.B[j], y[j]); y[j] = map_at(all.P[j], all.B[j], y[j]); }
         }
-      }
-      if (!MAPS) {
-        if (on) op.run(seg, in);
-        if (s.tls == 1) {
+      } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) y[j] = in[j];
-        }
+        for (int j = 0; j < VEC; ++j) y[j] = map_at(m.P[j], m.B[j], y[j]);
       }
+      if (!MAPS && on) op.write(place(k0), e);
     }
-    if (s.tl == 0 && nv) {
-      if (MAPS) { store_pack<float, VEC>(work + q * sh.columns + c0, run.P, nv); store_pack<float, VEC>(work + (sh.chunks + q) * sh.columns + c0, run.B, nv); }
-      else if (end && stop == sh.segments) store_pack<float, VEC>(end + c0, y, nv);
+    if (s.tl == 0 && there) {
+      if (MAPS) { store_pack<float, VEC>(work + q * sh.columns + c0, run.P); store_pack<float, VEC>(work + (sh.chunks + q) * sh.columns + c0, run.B); }
+      else if (end && stop == sh.segments) store_pack<float, VEC>(end + c0, y);
     }
   }
 }

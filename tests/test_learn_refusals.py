@@ -180,5 +180,7 @@ def test_c_entries_refuse_null_and_fail_loudly_without_a_gpu(lib):
 
 
 def test_nothing_to_do_is_no_error(lib):
+    assert lib.agarcl_recurrence_work(0, 3, 4) == lib.agarcl_recurrence_work(3, 0, 4) == lib.agarcl_recurrence_work(3, 4, 0) == lib.agarcl_advantages_work(0, 5) == 0
+    assert all(lib.agarcl_recurrence_work(t, b, c) >= 0 for t in (1, 8, 9, 100, 30000) for b in (1, 3, 5000) for c in (1, 2, 7, 256))
     for name, args in (("agarcl_recurrence", rec(rows=0)), ("agarcl_recurrence_grad", rec(width=0)), ("agarcl_advantages", adv(steps=0)), ("agarcl_sample_actions", sam(rows=0))):
         assert getattr(lib, name)(ctypes.byref(args)) == 0, name
