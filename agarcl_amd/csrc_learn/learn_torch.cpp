@@ -3,6 +3,9 @@
 // In C++ because these calls sit between two steps of the env: checks, structures, and above all a backward pass that would have to take Python's lock in autograd's own thread took
 // 23-155 us of host time per call from Python, a multiple of the kernels.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
@@ -13,8 +16,7 @@
 
 namespace py = pybind11;
 using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::Variable;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 namespace {
@@ -66,8 +68,6 @@ Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor &ref) { ret
 Tensor floats(at::IntArrayRef shape, const Tensor &ref) { return make(shape, at::kFloat, ref); }
 Tensor scratch(int64_t n, const Tensor &ref) { if (n < 0) refuse("sizes out of range"); return n ? floats({n}, ref) : Tensor(); }
 
-std::optional<Tensor> maybe(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
-
 // a tensor with every t[i] contiguous, and the elements from one index of the first axis to the next; a copy only where it has to be one
 struct Strided { Tensor t; int64_t stride = 0; };
 Strided steps(const Tensor &t) {
@@ -116,29 +116,31 @@ Remembered recurrence_forward(const Tensor &x, const Tensor &gate, const Tensor 
 
 void no_second_gradient() { if (at::GradMode::is_enabled()) throw std::runtime_error("agarcl_amd.learn has no gradients of gradients: call backward() / grad() without create_graph"); }
 
-struct RecurrenceFunction : torch::autograd::Function<RecurrenceFunction> {
-  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &gate, const std::optional<Tensor> &state, const std::optional<Tensor> &reset_) {
-    ctx->set_materialize_grads(false);
-    const Tensor reset = reset_.value_or(Tensor());
-    Remembered r = recurrence_forward(x, gate, state.value_or(Tensor()), reset, true);
-    ctx->save_for_backward({x, gate, reset, r.marks});
-    ctx->saved_data["state"] = state.has_value();
-    return {r.h, r.last};
+// A node of autograd's graph: what a backward pass reads is kept as SavedVariables, which notice a tensor that has been written since.
+struct RecurrenceNode : torch::autograd::Node {
+  SavedVariable x_, gate_, reset_, marks_;
+  void keep(const Tensor &x, const Tensor &gate, const Tensor &reset, const Tensor &marks) {
+    x_ = SavedVariable(x, false); gate_ = SavedVariable(gate, false); reset_ = SavedVariable(reset, false); marks_ = SavedVariable(marks, false);
   }
-  static variable_list backward(AutogradContext *ctx, const variable_list &up) {
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x_.reset_data(); gate_.reset_data(); reset_.reset_data(); marks_.reset_data();
+  }
+  variable_list apply(variable_list &&up) override {
+    std::lock_guard<std::mutex> lock(mutex_);
     no_second_gradient();
-    if (!up[0].defined() && !up[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0];
-    const Strided xs = steps(x), gs = steps(saved[1]), rs = steps(saved[2]), ds = steps(up[0]);
+    if (!up[0].defined() && !up[1].defined()) return variable_list(3);
+    const Tensor x = x_.unpack(), gate = gate_.unpack(), reset = reset_.unpack(), marks = marks_.unpack();
+    const Strided xs = steps(x), gs = steps(gate), rs = steps(reset), ds = steps(up[0]);
     const Tensor dlast = whole(up[1]);
     agarcl_recurrence_args a = recurrence_args(x, x.sizes(), xs, gs, rs);
     Tensor dx = make(x.sizes(), x.scalar_type(), x), dgate = make(x.sizes(), x.scalar_type(), x), dstate = floats(x.sizes().slice(1), x);
     const Tensor work = scratch(agarcl_recurrence_work(a.steps, a.rows, a.width), x);
-    a.marks = (float *)out(saved[3]); a.dh = ptr(ds.t); a.dh_stride = ds.stride; a.dlast = (const float *)ptr(dlast);
+    a.marks = (float *)out(marks); a.dh = ptr(ds.t); a.dh_stride = ds.stride; a.dlast = (const float *)ptr(dlast);
     a.dx = out(dx); a.dgate = out(dgate); a.dstate = (float *)out(dstate); a.work = (float *)out(work);
     done(agarcl_recurrence_grad(&a));
-    return {dx, dgate, ctx->saved_data["state"].toBool() ? dstate : Tensor(), Tensor()};
+    const auto wanted = [&](size_t i, Tensor &t) { return task_should_compute_output(i) ? t : Tensor(); };
+    return {wanted(0, dx), wanted(1, dgate), wanted(2, dstate)};
   }
 };
 
@@ -151,8 +153,17 @@ py::tuple gated_recurrence(py::handle hx, py::handle hgate, py::handle hstate, p
   if (reset.defined()) like(reset, "reset", x, FLAGS, x.sizes().slice(0, x.dim() - 1));
   on_gpu(x);
   if (at::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || (state.defined() && state.requires_grad()))) {
-    variable_list r = RecurrenceFunction::apply(x, gate, maybe(state), maybe(reset));
-    return py::make_tuple(r[0], r[1]);
+    auto node = std::shared_ptr<RecurrenceNode>(new RecurrenceNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, gate, state));
+    Remembered r;
+    {
+      at::NoGradGuard off;
+      r = recurrence_forward(x, gate, state, reset, true);
+    }
+    node->keep(x, gate, reset, r.marks);
+    torch::autograd::set_history(r.h, node);
+    torch::autograd::set_history(r.last, node);
+    return py::make_tuple(r.h, r.last);
   }
   Remembered r = recurrence_forward(x, gate, state, reset, false);
   return py::make_tuple(r.h, r.last);
@@ -296,41 +307,46 @@ Tensor loss_forward(const Tensor &logits, const Tensor &mean, const Tensor &log_
 // loss.  The first backward pass hands them out after its kernel has looked at the upstream gradient: it does nothing where that is 1 and works the
 // gradients out from the logits otherwise.  Every other backward pass (a second one through a kept graph; one that is captured: its replays may bring other
 // upstream gradients) works them out, into tensors of its own.  In float16 a loss is scaled as a rule, so there the forward pass leaves them.
-struct PolicyLossFunction : torch::autograd::Function<PolicyLossFunction> {
-  static Tensor forward(AutogradContext *ctx, const Tensor &logits, const std::optional<Tensor> &mean_, const std::optional<Tensor> &std_, LossCall *c) {
-    const Tensor mean = mean_.value_or(Tensor()), log_std = std_.value_or(Tensor());
-    Tensor g[3], std_one;
-    const bool ahead = logits.scalar_type() != at::kHalf && !capturing(logits);
-    if (ahead) loss_grads(*c, logits, mean, log_std, g);
-    if (c->need[2] && !c->per_row) std_one = floats({2}, logits);
-    const Tensor loss = loss_forward(logits, mean, log_std, *c, g, std_one);
-    if (ahead) { static const char *const names[3] = {"0", "1", "2"}; for (int i = 0; i < 3; ++i) if (g[i].defined()) ctx->saved_data[names[i]] = g[i]; }
-    ctx->saved_data["ahead"] = ahead;
-    ctx->saved_data["numbers"] = std::vector<double>{c->low, c->high, c->kl, c->entropy, (double)c->over, (double)c->per_row, (double)c->need[0], (double)c->need[1], (double)c->need[2]};
-    ctx->save_for_backward({logits, mean, log_std, c->stats, std_one, c->kind, c->old, c->adv, c->move, c->ref, c->allowed, c->weight});
-    return loss;
+struct PolicyLossNode : torch::autograd::Node {
+  SavedVariable in_[3], fixed_[7], stats_, std_one_;
+  LossCall c;                     // without its tensors
+  Tensor ahead_[3];               // the gradients for an upstream gradient of 1
+  bool ahead = false;
+  void keep(const Tensor &logits, const Tensor &mean, const Tensor &log_std, LossCall &call, const Tensor &std_one) {
+    const Tensor *in[3] = {&logits, &mean, &log_std}, *fixed[7] = {&call.kind, &call.old, &call.adv, &call.move, &call.ref, &call.allowed, &call.weight};
+    for (int i = 0; i < 3; ++i) in_[i] = SavedVariable(*in[i], false);
+    for (int i = 0; i < 7; ++i) fixed_[i] = SavedVariable(*fixed[i], false);
+    stats_ = SavedVariable(call.stats, false); std_one_ = SavedVariable(std_one, false);
+    c = LossCall{{}, {}, {}, {}, {}, {}, {}, call.low, call.high, call.kl, call.entropy, call.over, call.per_row, {call.need[0], call.need[1], call.need[2]}, {}};
   }
-  static variable_list backward(AutogradContext *ctx, const variable_list &up) {
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto &s : in_) s.reset_data();
+    for (auto &s : fixed_) s.reset_data();
+    stats_.reset_data(); std_one_.reset_data();
+    for (auto &t : ahead_) t.reset();
+    ahead = false;
+  }
+  variable_list apply(variable_list &&up) override {
+    std::lock_guard<std::mutex> lock(mutex_);
     no_second_gradient();
-    const variable_list s = ctx->get_saved_variables();
-    const Tensor &logits = s[0], &mean = s[1], &log_std = s[2], &std_one = s[4];
-    const std::vector<double> n = ctx->saved_data["numbers"].toDoubleVector();
-    LossCall c{s[5], s[6], s[7], s[8], s[9], s[10], s[11], n[0], n[1], n[2], n[3], (int)n[4], (int)n[5], {n[6] != 0, n[7] != 0, n[8] != 0}, s[3]};
+    if (!up[0].defined()) return variable_list(3);
+    const Tensor logits = in_[0].unpack(), mean = in_[1].unpack(), log_std = in_[2].unpack(), stats = stats_.unpack(), std_one = std_one_.unpack();
+    LossCall now{fixed_[0].unpack(), fixed_[1].unpack(), fixed_[2].unpack(), fixed_[3].unpack(), fixed_[4].unpack(), fixed_[5].unpack(), fixed_[6].unpack(), c.low, c.high, c.kl, c.entropy,
+                 c.over, c.per_row, {c.need[0], c.need[1], c.need[2]}, stats};
     std::vector<Tensor> kept;
-    agarcl_policy_loss_args a = loss_args(logits, mean, log_std, c, kept);
+    agarcl_policy_loss_args a = loss_args(logits, mean, log_std, now, kept);
     const Tensor upstream = up[0].to(at::kFloat).contiguous();
     Tensor g[3];
-    if (ctx->saved_data["ahead"].toBool() && !capturing(logits)) {
-      a.skip_if_one = 1;
-      const char *const names[3] = {"0", "1", "2"};
-      for (int i = 0; i < 3; ++i) { auto it = ctx->saved_data.find(names[i]); if (it != ctx->saved_data.end()) { g[i] = it->second.toTensor(); ctx->saved_data.erase(it); } }
-      ctx->saved_data["ahead"] = false;
-    } else loss_grads(c, logits, mean, log_std, g);
+    if (ahead && !capturing(logits)) {
+      a.skip_if_one = 1; ahead = false;
+      for (int i = 0; i < 3; ++i) g[i] = std::move(ahead_[i]);
+    } else loss_grads(now, logits, mean, log_std, g);
     if (c.need[2] && !c.per_row) g[2] = floats({2}, logits);
-    a.upstream = (const float *)ptr(upstream); a.weight_sum = (const float *)ptr(s[3]) + 4;
+    a.upstream = (const float *)ptr(upstream); a.weight_sum = (const float *)ptr(stats) + 4;
     a.dlogits = out(g[0]); a.dmean = out(g[1]); a.dlog_std = out(g[2]); a.dlog_std_one = (const float *)ptr(std_one);
     done(agarcl_policy_loss(&a));
-    return {g[0], g[1], g[2], Tensor()};
+    return {g[0], g[1], g[2]};
   }
 };
 
@@ -358,7 +374,18 @@ py::tuple policy_loss(py::handle hlogits, py::handle hkind, py::handle hold, py:
   c.need[0] = logits.requires_grad(); c.need[1] = mean.defined() && mean.requires_grad(); c.need[2] = log_std.defined() && log_std.requires_grad();
   Tensor loss;
   if (at::GradMode::is_enabled() && (c.need[0] || c.need[1] || c.need[2])) {
-    loss = PolicyLossFunction::apply(logits, maybe(mean), maybe(log_std), &c);
+    auto node = std::shared_ptr<PolicyLossNode>(new PolicyLossNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits, mean, log_std));
+    Tensor std_one;
+    {
+      at::NoGradGuard off;
+      node->ahead = logits.scalar_type() != at::kHalf && !capturing(logits);
+      if (node->ahead) loss_grads(c, logits, mean, log_std, node->ahead_);
+      if (c.need[2] && !c.per_row) std_one = floats({2}, logits);
+      loss = loss_forward(logits, mean, log_std, c, node->ahead_, std_one);
+    }
+    node->keep(logits, mean, log_std, c, std_one);
+    torch::autograd::set_history(loss, node);
   } else loss = loss_forward(logits, mean, log_std, c, {}, {});
   return py::make_tuple(loss, c.stats.select(0, 0), c.stats.select(0, 1), c.stats.select(0, 2), c.stats.select(0, 3));
 }
