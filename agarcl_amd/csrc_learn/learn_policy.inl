@@ -1,9 +1,9 @@
 // learn_policy.inl -- the clipped policy loss with its gradients, and the sampling of actions.
 //
-// Both are one pass over the logits: a row is in registers (or, beyond 32768 kinds, read twice) while its maximum, the sum s of e^(z - max) and
+// Both are one pass over the logits: a row is in registers (or, beyond 8192 kinds, read twice) while its maximum, the sum s of e^(z - max) and
 // u = sum of e^(z - max) (z - max) are taken; log s and u / s give the log-probabilities and the entropy, and the gradient is written from the same registers:
-// reading the logits once and writing their gradient once is all the memory traffic there has to be.  Up to 8 kinds a row is one thread's, up to 1024
-// a group of 2 to 64 lanes', beyond that a workgroup's.
+// reading the logits once and writing their gradient once is all the memory traffic there has to be.  Up to 8 kinds a row is one thread's, up to 2048
+// a group of 1 to 64 lanes', beyond that a workgroup's.
 
 static const int kLossBlocks = 2048, kWeightBlocks = 256;
 static const int64_t kLossWork = 8 * kLossBlocks + kWeightBlocks;
@@ -18,7 +18,7 @@ __global__ __launch_bounds__(256) void k_weight_sum(const float *__restrict__ w,
   double s = 0;
   int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   for (; i + 4 <= rows; i += (int64_t)gridDim.x * 1024) {
-    Raw<float, 4> r; load_raw<float, 4>(r, w + i, 4);
+    Raw<float, 4> r; load_raw<float, 4>(r, w + i);
     s += ((double)r[0] + (double)r[1]) + ((double)r[2] + (double)r[3]);
   }
   for (; i < rows; ++i) s += (double)w[i];      // (one thread's: the others' i is beyond rows, or their four were whole)
@@ -28,49 +28,37 @@ __global__ __launch_bounds__(256) void k_weight_sum(const float *__restrict__ w,
   if (threadIdx.x == 0) out[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
-// VE neighbouring logits of a row, still as they were loaded; what is not allowed, or not there, is made -inf in place, once, so that nothing after it
-// needs to know
+// VE neighbouring logits of a row, still as they were loaded; what is not allowed is made -inf in place, once, so that nothing after it needs to know
 template <class T, int VE> struct Kinds {
   Raw<T, VE> raw; uint32_t ok[(VE + 3) / 4];
-  __device__ __forceinline__ void load(const T *z, const uint8_t *allowed, int nv) {
-    load_raw<T, VE>(raw, z, nv);
+  __device__ __forceinline__ void load(const T *z, const uint8_t *allowed) {
+    load_raw<T, VE>(raw, z);
     if (allowed) {
       struct __attribute__((packed)) Bytes { uint8_t b[VE]; };
-      if (nv == VE) { ok[(VE - 1) / 4] = 0; __builtin_memcpy(ok, (const Bytes *)allowed, VE); }
-      else {
-#pragma unroll
-        for (int k = 0; k < VE; k += 4) {
-          ok[k / 4] = 0;
-#pragma unroll
-          for (int i = 0; i < 4 && k + i < VE; ++i) if (k + i < nv) ok[k / 4] |= (uint32_t)allowed[k + i] << (8 * i);
-        }
-      }
+      ok[(VE - 1) / 4] = 0;
+      __builtin_memcpy(ok, (const Bytes *)allowed, VE);
     }
   }
-  __device__ __forceinline__ void mask(bool flags, int nv) {
-    if (flags) {
+  __device__ __forceinline__ void none() {
 #pragma unroll
-      for (int k = 0; k < VE; ++k) if constexpr (sizeof(T) == 4) {
-        if (!(ok[k / 4] >> (8 * (k % 4)) & 255u)) raw.w[k] = 0xff800000u;
-      }
-      if constexpr (sizeof(T) == 2) {      // two at a time: 0 / nonzero bytes to 0 / 0xffff halves
-        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-        const uint32_t none = std::is_same<T, bf16_t>::value ? 0xff80ff80u : 0xfc00fc00u;
+    for (auto &w : raw.w) w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, bf16_t>::value ? 0xff80ff80u : 0xfc00fc00u;
 #pragma unroll
-        for (int k = 0; k < (VE + 1) / 2; ++k) {
-          const uint32_t pair = __builtin_amdgcn_perm(0u, ok[k / 2], k & 1 ? 0x0c030c02u : 0x0c010c00u);
-          u16x2 h = __builtin_bit_cast(u16x2, pair);
-          h = (u16x2)(0) - __builtin_elementwise_min(h, (u16x2)(1));
-          const uint32_t m = __builtin_bit_cast(uint32_t, h);
-          raw.w[k] = (raw.w[k] & m) | (none & ~m);
-        }
-      }
-    }
-    if (nv < VE) {
+    for (auto &w : ok) w = 0;
+  }
+  __device__ __forceinline__ void mask() {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int k = 0; k < VE; ++k) if (k >= nv) {
-        if constexpr (sizeof(T) == 4) raw.w[k] = 0xff800000u;
-        else { const uint32_t none = std::is_same<T, bf16_t>::value ? 0xff80u : 0xfc00u; raw.w[k / 2] = k & 1 ? (raw.w[k / 2] & 0xffffu) | none << 16 : (raw.w[k / 2] & 0xffff0000u) | none; }
+      for (int k = 0; k < VE; ++k) raw.w[k] = ok[k / 4] >> (8 * (k % 4)) & 255u ? raw.w[k] : 0xff800000u;
+    } else {      // two at a time: 0 / nonzero bytes to 0 / 0xffff halves
+      typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+      const uint32_t none = std::is_same<T, bf16_t>::value ? 0xff80ff80u : 0xfc00fc00u;
+#pragma unroll
+      for (int k = 0; k < (VE + 1) / 2; ++k) {
+        const uint32_t pair = __builtin_amdgcn_perm(0u, ok[k / 2], k & 1 ? 0x0c030c02u : 0x0c010c00u);
+        u16x2 h = __builtin_bit_cast(u16x2, pair);
+        h = (u16x2)(0) - __builtin_elementwise_min(h, (u16x2)(1));
+        const uint32_t m = __builtin_bit_cast(uint32_t, h);
+        raw.w[k] = (raw.w[k] & m) | (none & ~m);
       }
     }
   }
@@ -79,8 +67,8 @@ template <class T, int VE> struct Kinds {
 
 // what a row's kinds come to, relative to the maximum m: s = sum of e^(z - m), u = sum of e^(z - m) (z - m)
 struct RowSums { float m, s, u; };
-// z - m, and nothing so low that the product with e^(z - m) = 0 would not be 0
-// (the maximum that passes a NaN on: a NaN among the logits is to be seen in the loss)
+// z - m, and nothing so low that the product with e^(z - m) = 0 would not be 0.  (The maximum that passes a NaN on: a NaN among the logits is to be seen in the
+// loss.  And the difference before the factor log2 e: one multiply-add of both, 2 % faster, overflows where a mask is the type's lowest value.)
 __device__ __forceinline__ float below(float z, float m) { return __builtin_elementwise_maximum(z - m, -200.f); }
 // the reference point of a row: its maximum, or anything finite where nothing is allowed
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
@@ -91,73 +79,90 @@ __device__ __forceinline__ void sums_shift(RowSums &r, float m) {
   r.m = m;
 }
 
-// everything of a row that is not per kind
-struct LossRow { bool counts; int32_t kind; float sg, c0, c1; };      // dlogit[j] = p[j] (c1 (z[j] - m) + c0) + (j == kind ? sg : 0)
+// what of a row is not per kind, loaded ahead of its logits
+struct RowIn { float w, A, old, ref, za; int32_t kind; bool counts; };
+template <class T> __device__ __forceinline__ RowIn row_in(const agarcl_policy_loss_args &a, int64_t row) {
+  RowIn r;
+  r.kind = a.kind[row]; r.w = a.weight ? a.weight[row] : 1.f; r.A = a.advantage[row]; r.old = a.old_log_prob[row]; r.ref = a.ref_log_prob ? a.ref_log_prob[row] : r.old;
+  return r;
+}
+template <class T> __device__ __forceinline__ void row_kind(const agarcl_policy_loss_args &a, RowIn &r, const T *z, const uint8_t *ok) {      // (its kind's own logit)
+  r.counts = r.w != 0.f && r.kind >= 0 && r.kind < a.kinds;
+  const int32_t k = r.counts ? r.kind : 0;
+  r.za = to_f(z[k]);
+  r.counts = r.counts && r.za != -INFINITY && (!ok || ok[k]);
+}
+
+// dlogit[j] = e^d[j] (c1 d[j] + c0) + (j == kind ? sg : 0), d[j] = z[j] - m
+struct LossRow { float sg, c0, c1; };
 struct LossTotals { float inv; bool shared_std; };
 
-template <class T> __device__ __forceinline__ LossRow loss_row(const agarcl_policy_loss_args &a, const LossTotals &t, int64_t row, const RowSums &r, const T *z, const uint8_t *ok,
-    bool leader, double (&acc)[7]) {
+// e^x - 1 and e^x - 1 - x: near 0, where both are the difference of near numbers, from the series (|x| < 0.35: 2e-8 of the value is left out)
+__device__ __forceinline__ void exp_less(float x, float &less1, float &less1x) {
+  const float p = fmaf(x, fmaf(x, fmaf(x, fmaf(x, fmaf(x, 1.f / 5040, 1.f / 720), 1.f / 120), 1.f / 24), 1.f / 6), 0.5f) * x * x, e = __expf(x) - 1.f;
+  const bool near = fabsf(x) < 0.35f;
+  less1x = near ? p : e - x; less1 = near ? p + x : e;
+}
+
+template <class T> __device__ __forceinline__ LossRow loss_row(const agarcl_policy_loss_args &a, const LossTotals &t, int64_t row, const RowIn &in, const RowSums &r, bool leader,
+    float (&acc)[7]) {
   LossRow o;
-  const float w = a.weight ? a.weight[row] : 1.f, A = a.advantage[row], old = a.old_log_prob[row], ref = a.ref_log_prob ? a.ref_log_prob[row] : old;
-  const int32_t kind = o.kind = a.kind[row];
-  o.counts = w != 0.f && kind >= 0 && kind < a.kinds;
-  float za = 0.f;
-  if (o.counts) { za = to_f(z[kind]); o.counts = za != -INFINITY && (!ok || ok[kind]); }
-  const float log_s = logf(r.s), rs = 1.f / r.s, hcat = log_s - r.u * rs;
-  float lp = za - r.m - log_s, ent = hcat;
+  const float log_s = logf(r.s), rs = __builtin_amdgcn_rcpf(r.s), hcat = log_s - r.u * rs, A = in.A;
+  float lp = in.za - r.m - log_s, ent = hcat;
   float dev[2] = {0.f, 0.f}, istd[2] = {0.f, 0.f};
   if (a.mean) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
       const float ls = log_std_at<T>(a.log_std, a.log_std_per_row, row, d);
-      istd[d] = expf(-ls);
+      istd[d] = __expf(-ls);
       dev[d] = (a.move[2 * row + d] - to_f(((const T *)a.mean)[2 * row + d])) * istd[d];
       lp -= 0.5f * dev[d] * dev[d] + ls + kHalfLog2Pi;
       ent += ls + kHalfLog2PiE;
     }
   }
-  const float ratio = expf(lp - old);
-  const bool clipped = A >= 0.f ? ratio > 1.f + a.clip_high : ratio < 1.f - a.clip_low;
-  const float back = ref - lp, eb = expm1f(back);      // (expm1: near 0 the KL term is the difference of near numbers)
+  const float ratio = __expf(lp - in.old), high = 1.f + a.clip_high, lowest = 1.f - a.clip_low;
+  const bool clipped = A >= 0.f ? ratio > high : ratio < lowest;
+  float eb, kl;
+  exp_less(in.ref - lp, eb, kl);
   float g = clipped || A == 0.f ? 0.f : -A * ratio;
   if (a.kl_coef != 0.f) g -= a.kl_coef * eb;
-  const float share = w * t.inv, ce = a.entropy_coef;
+  const float share = in.w * t.inv, ce = a.entropy_coef;
   o.sg = share * g; o.c1 = share * ce * rs; o.c0 = (ce != 0.f ? share * ce * (hcat - log_s) - o.sg : -o.sg) * rs;
   if (leader) {
-    const float low = A == 0.f ? 0.f : fminf(ratio * A, fminf(fmaxf(ratio, 1.f - a.clip_low), 1.f + a.clip_high) * A);
-    acc[0] += (double)w;
-    if (o.counts) {
-      acc[1] += (double)w * low; acc[2] += (double)w * (eb - back); acc[3] += (double)w * ent; acc[4] += clipped ? (double)w : 0.;
+    const float low = A == 0.f ? 0.f : fminf(ratio * A, fminf(fmaxf(ratio, lowest), high) * A), w = in.w;
+    acc[0] += w;
+    if (in.counts) {
+      acc[1] += w * low; acc[2] += w * kl; acc[3] += w * ent; acc[4] += clipped ? w : 0.f;
       if (t.shared_std) {
 #pragma unroll
-        for (int d = 0; d < 2; ++d) acc[5 + d] += (double)w * (g * (dev[d] * dev[d] - 1.f) - ce);
+        for (int d = 0; d < 2; ++d) acc[5 + d] += w * (g * (dev[d] * dev[d] - 1.f) - ce);
       }
     }
     if (a.dmean) {
       float v[2];
 #pragma unroll
-      for (int d = 0; d < 2; ++d) v[d] = o.counts ? o.sg * dev[d] * istd[d] : 0.f;
-      store_pack<T, 2>((T *)a.dmean + 2 * row, v, 2);
+      for (int d = 0; d < 2; ++d) v[d] = in.counts ? o.sg * dev[d] * istd[d] : 0.f;
+      store_pack<T, 2>((T *)a.dmean + 2 * row, v);
     }
     if (a.dlog_std && a.log_std_per_row) {
       float v[2];
 #pragma unroll
-      for (int d = 0; d < 2; ++d) v[d] = o.counts ? o.sg * (dev[d] * dev[d] - 1.f) - share * ce : 0.f;
-      store_pack<T, 2>((T *)a.dlog_std + 2 * row, v, 2);
+      for (int d = 0; d < 2; ++d) v[d] = in.counts ? o.sg * (dev[d] * dev[d] - 1.f) - share * ce : 0.f;
+      store_pack<T, 2>((T *)a.dlog_std + 2 * row, v);
     }
   }
   return o;
 }
 
-// the gradient of kinds j0 ... of a row.  The probabilities are worked out once more: holding 8 of them for every 4 registers of logits would cost more
+// the gradient of kinds j0 ... of a row, into dz.  The probabilities are worked out once more: holding 8 of them for every 4 registers of logits would cost more
 // (registers, and with them wavefronts) than a second exp
-template <class T, int VE> __device__ __forceinline__ void loss_kinds(const agarcl_policy_loss_args &a, const LossRow &o, float m, int64_t row, int64_t j0, int nv, Kinds<T, VE> &z) {
+template <class T, int VE> __device__ __forceinline__ void loss_kinds(const RowIn &in, const LossRow &o, float m, int64_t j0, Kinds<T, VE> &z, T *dz) {
   z.raw.anew();
   float v[VE];
-  if (o.counts) {
+  if (in.counts) {
 #pragma unroll
     for (int k = 0; k < VE; ++k) { const float d = below(z[k], m); v[k] = __expf(d) * fmaf(o.c1, d, o.c0); }
-    const int64_t at = o.kind - j0;
+    const int64_t at = in.kind - j0;
     if (at >= 0 && at < VE) {
 #pragma unroll
       for (int k = 0; k < VE; ++k) v[k] += k == (int)at ? o.sg : 0.f;
@@ -166,7 +171,7 @@ template <class T, int VE> __device__ __forceinline__ void loss_kinds(const agar
 #pragma unroll
     for (int k = 0; k < VE; ++k) v[k] = 0.f;
   }
-  store_pack<T, VE>((T *)a.dlogits + row * a.kinds + j0, v, nv);
+  store_pack<T, VE>(dz + j0, v);
 }
 
 // what comes before the rows; false: there is nothing to do
@@ -198,10 +203,11 @@ __device__ __forceinline__ bool loss_begin(const agarcl_policy_loss_args &a, Los
   }
   return true;
 }
-__device__ __forceinline__ void loss_end(const agarcl_policy_loss_args &a, double (&acc)[7], double *lds) {
+// the workgroup's sums.  A thread adds up its own few rows in 32 bits, everything above that is added in 64
+__device__ __forceinline__ void loss_end(const agarcl_policy_loss_args &a, const float (&acc)[7], double *lds) {
   if (!a.want_stats) return;
 #pragma unroll
-  for (int i = 0; i < 7; ++i) { const double s = wave_sum(acc[i]); if ((threadIdx.x & 63) == 0) lds[8 * (threadIdx.x >> 6) + i] = s; }
+  for (int i = 0; i < 7; ++i) { const double s = wave_sum((double)acc[i]); if ((threadIdx.x & 63) == 0) lds[8 * (threadIdx.x >> 6) + i] = s; }
   __syncthreads();
   if (threadIdx.x < 7) {
     double s = 0;
@@ -216,39 +222,46 @@ __global__ __launch_bounds__(256) void k_loss_thread(const agarcl_policy_loss_ar
   __shared__ double lds[32];
   LossTotals t;
   if (!loss_begin(a, t, lds)) return;
-  double acc[7] = {0, 0, 0, 0, 0, 0, 0};
+  float acc[7] = {0, 0, 0, 0, 0, 0, 0};
   for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) {
     const T *zp = (const T *)a.logits + row * a.logits_stride;
     const uint8_t *ok = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-    Kinds<T, V> z; z.load(zp, ok, V); z.mask(ok, V);
+    RowIn in = row_in<T>(a, row);
+    Kinds<T, V> z; z.load(zp, ok);
+    row_kind<T>(a, in, zp, ok);
+    if (ok) z.mask();
     RowSums r = {-INFINITY, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < V; ++k) r.m = fmaxf(r.m, z[k]);
     r.m = finite_max(r.m);
 #pragma unroll
     for (int k = 0; k < V; ++k) sums_add(r, z[k]);
-    const LossRow o = loss_row<T>(a, t, row, r, zp, ok, true, acc);
-    if (a.dlogits) loss_kinds<T, V>(a, o, r.m, row, 0, V, z);
+    const LossRow o = loss_row<T>(a, t, row, in, r, true, acc);
+    if (a.dlogits) loss_kinds<T, V>(in, o, r.m, 0, z, (T *)a.dlogits + row * a.kinds);
   }
   loss_end(a, acc, lds);
 }
 
-// a thread's CHUNKS x 8 kinds of a row, chunk c at j0 + c x stride
+// a thread's chunks of 8 kinds of a row (of 8 kinds or more).  The row's last chunk begins 8 kinds before its end: the kinds that the chunk before it has, too,
+// are left out of the sums (skip of them) and get the same gradient from both.
 template <class T, int CHUNKS> struct Share {
-  Kinds<T, 8> z[CHUNKS]; int nv[CHUNKS];
+  Kinds<T, 8> z[CHUNKS]; int32_t skip[CHUNKS]; uint32_t there;
+  __device__ __forceinline__ static int64_t begin(int64_t j, int64_t kinds) { return j + 8 <= kinds ? j : kinds - 8; }
   __device__ __forceinline__ void load(const T *zp, const uint8_t *ok, int64_t j0, int64_t stride, int64_t kinds, bool on) {
+    there = 0;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      const int64_t j = j0 + c * stride, left = kinds - j;
-      nv[c] = on ? (left < 0 ? 0 : left < 8 ? (int)left : 8) : 0;
-      z[c].load(zp + j, ok ? ok + j : nullptr, nv[c]);
+      const int64_t j = j0 + c * stride, b = begin(j, kinds);
+      skip[c] = (int32_t)(j - b);
+      if (on && j < kinds) { there |= 1u << c; z[c].load(zp + b, ok ? ok + b : nullptr); }
+      else z[c].none();
     }
   }
   __device__ __forceinline__ float top(bool flags) {
     float m = -INFINITY;
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      z[c].mask(flags, nv[c]);
+      if (flags) z[c].mask();
 #pragma unroll
       for (int k = 0; k < 8; ++k) m = fmaxf(m, z[c][k]);
       __builtin_amdgcn_sched_barrier(0);      // (chunk after chunk: all at once would take the registers of a second wavefront)
@@ -259,42 +272,49 @@ template <class T, int CHUNKS> struct Share {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
       z[c].raw.anew();
+      if (__any(skip[c] > 0 && (there >> c & 1))) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sums_add(r, z[c][k]);
+        for (int k = 0; k < 8; ++k) sums_add(r, k < skip[c] ? -INFINITY : z[c][k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sums_add(r, z[c][k]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   }
-  __device__ __forceinline__ void gradient(const agarcl_policy_loss_args &a, const LossRow &o, float m, int64_t row, int64_t j0, int64_t stride) {
+  __device__ __forceinline__ void gradient(const RowIn &in, const LossRow &o, float m, int64_t j0, int64_t stride, T *dz) {
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      if (nv[c] > 0) loss_kinds<T, 8>(a, o, m, row, j0 + c * stride, nv[c], z[c]);
+      if (there >> c & 1) loss_kinds<T, 8>(in, o, m, j0 + c * stride - skip[c], z[c], dz);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
 
-// 8 << g_log (x CHUNKS) kinds, a group of 1 << g_log lanes per row
+// CHUNKS x 8 << g_log kinds, a group of 1 << g_log lanes per row
 template <class T, int CHUNKS>
 __global__ __launch_bounds__(256) void k_loss_lanes(const agarcl_policy_loss_args a, const int g_log) {
   __shared__ double lds[32];
   LossTotals t;
   if (!loss_begin(a, t, lds)) return;
-  double acc[7] = {0, 0, 0, 0, 0, 0, 0};
+  float acc[7] = {0, 0, 0, 0, 0, 0, 0};
   const int g = 1 << g_log, lane = threadIdx.x & (g - 1), per = 256 >> g_log;
   for (int64_t first = (int64_t)blockIdx.x * per; first < a.rows; first += (int64_t)gridDim.x * per) {
-    const int64_t row = first + (threadIdx.x >> g_log);
+    const int64_t row = first + (threadIdx.x >> g_log), safe = row < a.rows ? row : 0;
     const bool on = row < a.rows;
-    const T *zp = (const T *)a.logits + (on ? row : 0) * a.logits_stride;
-    const uint8_t *ok = a.allowed ? a.allowed + (on ? row : 0) * a.allowed_stride : nullptr;
+    const T *zp = (const T *)a.logits + safe * a.logits_stride;
+    const uint8_t *ok = a.allowed ? a.allowed + safe * a.allowed_stride : nullptr;
+    RowIn in = row_in<T>(a, safe);
     Share<T, CHUNKS> z; z.load(zp, ok, lane * 8, g * 8, a.kinds, on);
+    row_kind<T>(a, in, zp, ok);
     RowSums r = {z.top(ok), 0.f, 0.f};
     for (int d = 1; d < g; d <<= 1) r.m = fmaxf(r.m, __shfl_xor(r.m, d));
     r.m = finite_max(r.m);
     z.sum(r);
     for (int d = 1; d < g; d <<= 1) { r.s += __shfl_xor(r.s, d); r.u += __shfl_xor(r.u, d); }
     if (!on) continue;      // (a whole group, behind the last of the shuffles of this turn)
-    const LossRow o = loss_row<T>(a, t, row, r, zp, ok, lane == 0, acc);
-    if (a.dlogits) z.gradient(a, o, r.m, row, lane * 8, g * 8);
+    const LossRow o = loss_row<T>(a, t, row, in, r, lane == 0, acc);
+    if (a.dlogits) z.gradient(in, o, r.m, lane * 8, g * 8, (T *)a.dlogits + row * a.kinds);
   }
   loss_end(a, acc, lds);
 }
@@ -324,44 +344,50 @@ __global__ __launch_bounds__(NT) void k_loss_block(const agarcl_policy_loss_args
   __shared__ float wl[2][NT / 64][4];
   LossTotals t;
   if (!loss_begin(a, t, lds)) return;
-  double acc[7] = {0, 0, 0, 0, 0, 0, 0};
+  float acc[7] = {0, 0, 0, 0, 0, 0, 0};
   int parity = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
     const T *zp = (const T *)a.logits + row * a.logits_stride;
     const uint8_t *ok = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+    T *dz = (T *)a.dlogits + row * a.kinds;
+    RowIn in = row_in<T>(a, row);
     if constexpr (CHUNKS > 0) {
       Share<T, CHUNKS> z; z.load(zp, ok, threadIdx.x * 8, NT * 8, a.kinds, true);
+      row_kind<T>(a, in, zp, ok);
       const float top = wave_max(z.top(ok));
       RowSums r = {finite_max(top), 0.f, 0.f};
       z.sum(r);
       r.s = wave_sum(r.s); r.u = wave_sum(r.u);
       r.m = top;
       const RowSums all = join_waves<NT>(r, wl, parity);
-      const LossRow o = loss_row<T>(a, t, row, all, zp, ok, threadIdx.x == 0, acc);
-      if (a.dlogits) z.gradient(a, o, all.m, row, threadIdx.x * 8, NT * 8);
+      const LossRow o = loss_row<T>(a, t, row, in, all, threadIdx.x == 0, acc);
+      if (a.dlogits) z.gradient(in, o, all.m, threadIdx.x * 8, NT * 8, dz);
     } else {
+      row_kind<T>(a, in, zp, ok);
       RowSums r = {-INFINITY, 0.f, 0.f};
       for (int64_t j0 = (int64_t)threadIdx.x * 8; j0 < a.kinds; j0 += NT * 8) {
-        const int nv = a.kinds - j0 < 8 ? (int)(a.kinds - j0) : 8;
-        Kinds<T, 8> z; z.load(zp + j0, ok ? ok + j0 : nullptr, nv); z.mask(ok, nv);
+        const int64_t b = Share<T, 1>::begin(j0, a.kinds);
+        Kinds<T, 8> z; z.load(zp + b, ok ? ok + b : nullptr);
+        if (ok) z.mask();
         float m = r.m;
 #pragma unroll
         for (int k = 0; k < 8; ++k) m = fmaxf(m, z[k]);
         sums_shift(r, m);
         RowSums c = {finite_max(m), 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sums_add(c, z[k]);
+        for (int k = 0; k < 8; ++k) sums_add(c, k < (int)(j0 - b) ? -INFINITY : z[k]);
         r.s += c.s; r.u += c.u;
       }
       sums_shift(r, wave_max(r.m));
       r.s = wave_sum(r.s); r.u = wave_sum(r.u);
       const RowSums all = join_waves<NT>(r, wl, parity);
-      const LossRow o = loss_row<T>(a, t, row, all, zp, ok, threadIdx.x == 0, acc);
+      const LossRow o = loss_row<T>(a, t, row, in, all, threadIdx.x == 0, acc);
       if (a.dlogits) {
         for (int64_t j0 = (int64_t)threadIdx.x * 8; j0 < a.kinds; j0 += NT * 8) {
-          const int nv = a.kinds - j0 < 8 ? (int)(a.kinds - j0) : 8;
-          Kinds<T, 8> z; z.load(zp + j0, ok ? ok + j0 : nullptr, nv); z.mask(ok, nv);
-          loss_kinds<T, 8>(a, o, all.m, row, j0, nv, z);
+          const int64_t b = Share<T, 1>::begin(j0, a.kinds);
+          Kinds<T, 8> z; z.load(zp + b, ok ? ok + b : nullptr);
+          if (ok) z.mask();
+          loss_kinds<T, 8>(in, o, all.m, b, z, dz);
         }
       }
     }
@@ -391,31 +417,34 @@ __global__ __launch_bounds__(512) void k_loss_stats(const agarcl_policy_loss_arg
   if (a.dlog_std && !a.log_std_per_row) for (int d = 0; d < 2; ++d) ((float *)a.dlog_std)[d] = (float)(sums[5 + d] * by);
 }
 
-// how many kinds call for which kernel; the workgroups a launch needs
-static unsigned loss_grid(int64_t rows, int64_t per) { const int64_t n = (rows + per - 1) / per; return (unsigned)(n < kLossBlocks ? n : kLossBlocks); }
+// How many kinds call for which kernel.  What a row needs besides its kinds (a logarithm, exponentials, the sums over its lanes) is a few hundred instructions of every
+// wavefront that works on it, so lanes hold several chunks: 65536 rows of 500 bf16 kinds with 64 / 32 / 16 lanes of 1 / 2 / 4 chunks 112 / 56 / 48 us, 300000 of 64 with
+// 8 / 4 / 2 lanes 31 / 25 / 27; 8209 rows of 6144 with 128 threads of 6 chunks 67 us, 256 of 3 76, 1024 of 1 172.  A workgroup of 256 that reads a row twice: 16384 kinds
+// 58 us, where 1024 threads that hold it took 74.
+static unsigned loss_grid(int64_t rows, int64_t per, int64_t most) { const int64_t n = (rows + per - 1) / per; return (unsigned)(n < most ? n : most); }
 template <class T> static unsigned loss_launch(const agarcl_policy_loss_args &a, hipStream_t st) {
   const int64_t V = a.kinds;
   unsigned grid;
   if (V <= 8) {
-    grid = loss_grid(a.rows, 256);
+    grid = loss_grid(a.rows, 256, kLossBlocks / 2);
     switch ((int)V) {
 #define ONE(n) case n: k_loss_thread<T, n><<<dim3(grid), 256, 0, st>>>(a); break;
       ONE(1) ONE(2) ONE(3) ONE(4) ONE(5) ONE(6) ONE(7) ONE(8)
 #undef ONE
     }
-  } else if (V <= 1024) {
-    int g_log = 1;
-    while (g_log < 6 && (8 << g_log) < V) ++g_log;
-    grid = loss_grid(a.rows, 256 >> g_log);
-    if (V <= 512) k_loss_lanes<T, 1><<<dim3(grid), 256, 0, st>>>(a, g_log);
-    else k_loss_lanes<T, 2><<<dim3(grid), 256, 0, st>>>(a, g_log);
+  } else if (V <= 2048) {
+    const int chunks = V <= 128 ? 2 : 4;
+    int g_log = 0;
+    while ((chunks * 8 << g_log) < V) ++g_log;
+    grid = loss_grid(a.rows, 256 >> g_log, kLossBlocks / 2);
+    if (chunks == 2) k_loss_lanes<T, 2><<<dim3(grid), 256, 0, st>>>(a, g_log);
+    else k_loss_lanes<T, 4><<<dim3(grid), 256, 0, st>>>(a, g_log);
   } else {
-    grid = loss_grid(a.rows, 1);
-    if (V <= 4096) k_loss_block<T, 256, 2><<<dim3(grid), 256, 0, st>>>(a);
-    else if (V <= 8192) k_loss_block<T, 256, 4><<<dim3(grid), 256, 0, st>>>(a);
-    else if (V <= 16384) k_loss_block<T, 1024, 2><<<dim3(grid), 1024, 0, st>>>(a);
-    else if (V <= 32768) k_loss_block<T, 1024, 4><<<dim3(grid), 1024, 0, st>>>(a);
-    else k_loss_block<T, 1024, 0><<<dim3(grid), 1024, 0, st>>>(a);
+    grid = loss_grid(a.rows, 1, kLossBlocks);
+    if (V <= 128 * 8 * 4) k_loss_block<T, 128, 4><<<dim3(grid), 128, 0, st>>>(a);
+    else if (V <= 128 * 8 * 6) k_loss_block<T, 128, 6><<<dim3(grid), 128, 0, st>>>(a);
+    else if (V <= 128 * 8 * 8) k_loss_block<T, 128, 8><<<dim3(grid), 128, 0, st>>>(a);
+    else k_loss_block<T, 256, 0><<<dim3(grid), 256, 0, st>>>(a);
   }
   return grid;
 }
@@ -426,10 +455,11 @@ static const int NONE = INT32_MAX;
 struct Pick { RowSums r; float best; int at; };
 __device__ __forceinline__ void pick_join(Pick &p, float best, int at) { if (at != NONE && (p.at == NONE || best > p.best || (best == p.best && at < p.at))) { p.best = best; p.at = at; } }
 
-template <class T, int VE> __device__ __forceinline__ void pick_kinds(Pick &p, const T *z, const uint8_t *ok, const float *gum, int64_t j0, int nv) {
-  Kinds<T, VE> k; k.load(z + j0, ok ? ok + j0 : nullptr, nv); k.mask(ok, nv);
+template <class T, int VE> __device__ __forceinline__ void pick_kinds(Pick &p, const T *z, const uint8_t *ok, const float *gum, int64_t j0, int skip) {
+  Kinds<T, VE> k; k.load(z + j0, ok ? ok + j0 : nullptr);
   Raw<float, VE> gu;
-  if (gum) load_raw<float, VE>(gu, gum + j0, nv);
+  if (gum) load_raw<float, VE>(gu, gum + j0);
+  if (ok) k.mask();
   float m = p.r.m;
 #pragma unroll
   for (int i = 0; i < VE; ++i) m = fmaxf(m, k[i]);
@@ -437,7 +467,7 @@ template <class T, int VE> __device__ __forceinline__ void pick_kinds(Pick &p, c
 #pragma unroll
   for (int i = 0; i < VE; ++i) {
     const float v = k[i];
-    if (v == -INFINITY) continue;
+    if (v == -INFINITY || i < skip) continue;
     p.r.s += __expf(below(v, m));
     const float score = gum ? v + gu[i] : v;
     if (p.at == NONE || score > p.best) { p.best = score; p.at = (int)(j0 + i); }      // (indices rise within a thread: the first of equals stays)
@@ -455,7 +485,7 @@ template <class T> __device__ __forceinline__ void pick_write(const agarcl_sampl
       move[d] = fminf(fmaxf(raw[d], -1.f), 1.f);
       lp -= 0.5f * n * n + ls + kHalfLog2Pi;
     }
-    store_pack<float, 2>(a.raw + 2 * row, raw, 2); store_pack<float, 2>(a.move + 2 * row, move, 2);
+    store_pack<float, 2>(a.raw + 2 * row, raw); store_pack<float, 2>(a.move + 2 * row, move);
   }
   a.log_prob[row] = lp;
 }
@@ -465,7 +495,7 @@ __global__ __launch_bounds__(256) void k_sample_thread(const agarcl_sample_args 
   for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) {
     const T *z = (const T *)a.logits + row * a.logits_stride;
     Pick p = {{-INFINITY, 0.f, 0.f}, -INFINITY, NONE};
-    pick_kinds<T, V>(p, z, a.allowed ? a.allowed + row * a.allowed_stride : nullptr, a.gumbel ? a.gumbel + row * a.gumbel_stride : nullptr, 0, V);
+    pick_kinds<T, V>(p, z, a.allowed ? a.allowed + row * a.allowed_stride : nullptr, a.gumbel ? a.gumbel + row * a.gumbel_stride : nullptr, 0, 0);
     pick_write<T>(a, row, p, z);
   }
 }
@@ -485,7 +515,10 @@ __global__ __launch_bounds__(256) void k_sample_lanes(const agarcl_sample_args a
     if (on) {
       const uint8_t *ok = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
       const float *gum = a.gumbel ? a.gumbel + row * a.gumbel_stride : nullptr;
-      for (int64_t j0 = (int64_t)lane * 8; j0 < a.kinds; j0 += (int64_t)g * 8) pick_kinds<T, 8>(p, z, ok, gum, j0, a.kinds - j0 < 8 ? (int)(a.kinds - j0) : 8);
+      for (int64_t j0 = (int64_t)lane * 8; j0 < a.kinds; j0 += (int64_t)g * 8) {
+        const int64_t b = Share<T, 1>::begin(j0, a.kinds);
+        pick_kinds<T, 8>(p, z, ok, gum, b, (int)(j0 - b));
+      }
     }
     float m = p.r.m;
     for (int d = 1; d < in_wave; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));

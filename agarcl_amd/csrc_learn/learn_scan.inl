@@ -40,17 +40,6 @@ template <class T, int VEC> __device__ __forceinline__ void load_raw(Raw<T, VEC>
   out.w[(VEC * sizeof(T) - 1) / 4] = 0;
   __builtin_memcpy(out.w, (const Pack<T, VEC> *)p, VEC * sizeof(T));
 }
-// the first nv of them; the others 0
-template <class T, int VEC> __device__ __forceinline__ void load_raw(Raw<T, VEC> &out, const T *p, int nv) {
-  if (nv == VEC) load_raw<T, VEC>(out, p);
-  else {
-#pragma unroll
-    for (int k = 0; k < (int)(VEC * sizeof(T) + 3) / 4; ++k) {
-      if constexpr (sizeof(T) == 4) out.w[k] = k < nv ? ((const uint32_t *)p)[k] : 0u;
-      else out.w[k] = (2 * k < nv ? (uint32_t)((const uint16_t *)p)[2 * k] : 0u) | (2 * k + 1 < nv ? (uint32_t)((const uint16_t *)p)[2 * k + 1] << 16 : 0u);
-    }
-  }
-}
 template <int VEC> __device__ __forceinline__ void load_floats(float (&out)[VEC], const float *p) {
   Raw<float, VEC> r; load_raw<float, VEC>(r, p);
 #pragma unroll
@@ -61,13 +50,6 @@ template <class T, int VEC> __device__ __forceinline__ void store_pack(T *p, con
 #pragma unroll
   for (int j = 0; j < VEC; ++j) k.v[j] = from_f<T>(in[j]);
   *(Pack<T, VEC> *)p = k;
-}
-template <class T, int VEC> __device__ __forceinline__ void store_pack(T *p, const float (&in)[VEC], int nv) {
-  if (nv == VEC) store_pack<T, VEC>(p, in);
-  else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) if (j < nv) p[j] = from_f<T>(in[j]);
-  }
 }
 // device memory at an address that is the same for the wavefront and an offset that is the lane's: the form that loads take without vector arithmetic
 template <class T> __device__ __forceinline__ T *device_ptr(uintptr_t base, uint32_t off) { return (T *)(GLOBAL T *)((GLOBAL char *)base + off); }
