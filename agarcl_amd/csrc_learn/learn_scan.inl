@@ -133,15 +133,16 @@ __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const 
     // neighbouring column groups share 128-byte lines where they are narrow: keep them on one XCD, behind one L2 (workgroups go to the 8 XCDs in turn)
     const int64_t group = sh.slots >= 16 ? (b & 7) * (sh.slots >> 3) + (b >> 3) : b;
     if (group >= sh.groups) continue;
-    const int64_t cbase = (group << sh.cl_log) * VEC;
-    int64_t c0 = cbase + s.col * VEC;
+    int64_t cbase = (group << sh.cl_log) * VEC, c0 = cbase + s.col * VEC;
     const bool there = c0 < sh.columns;
-    // (the last thread of a row of columns that VEC does not divide takes some of its neighbour's, too, and writes the same there)
+    // (the last thread of a row of columns that VEC does not divide takes some of its neighbour's, too, and writes the same there; where it is its workgroup's
+    // first, the workgroup begins there, or the offset from its beginning would be below 0)
+    if (cbase + VEC > sh.columns) cbase = sh.columns - VEC;
     if (there && c0 + VEC > sh.columns) c0 = sh.columns - VEC;
     op.start(there ? c0 : 0);
     // the turn that begins with segment k0 (counted in the scan's order)
     const auto place = [&](int64_t k0) __attribute__((always_inline)) {
-      return Place{(Op::reverse ? sh.segments - s.tls - k0 : k0) * SEG, cbase, (uint32_t)(Op::reverse ? s.tls - 1 - s.tl : s.tl) * SEG, (uint32_t)(c0 - cbase)};
+      return Place{(Op::reverse ? sh.segments - s.tls - k0 : k0) * SEG, cbase, (uint32_t)(Op::reverse ? s.tls - 1 - s.tl : s.tl) * SEG, there ? (uint32_t)(c0 - cbase) : 0u};
     };
     float y[VEC];
     Map<VEC> run; map_clear(run);
