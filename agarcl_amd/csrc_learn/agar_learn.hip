@@ -35,7 +35,9 @@ static bool type_ok(int32_t dt) { return dt == AGARCL_F32 || dt == AGARCL_BF16 |
 static const int64_t kMost = (int64_t)1 << 40;      // no dimension, stride or product of dimensions above this: 64-bit index arithmetic cannot overflow
 static bool sizes_ok(int64_t a, int64_t b, int64_t c) {
   if (a < 0 || b < 0 || c < 0 || a > kMost || b > kMost || c > kMost) return false;
-  if (a == 0 || b == 0 || c == 0) return true;
+  if (a == 0) a = 1;      // (the product of the others counts all the same)
+  if (b == 0) b = 1;
+  if (c == 0) c = 1;
   return a <= kMost / b && a * b <= kMost / c;
 }
 static bool stride_ok(int64_t s, int64_t steps, int64_t least) { return steps <= 1 || (s >= least && s <= kMost && s <= (kMost << 10) / steps); }
@@ -178,7 +180,7 @@ extern "C" int agarcl_policy_loss(const agarcl_policy_loss_args *a) {
     if (const int rc = launched("policy loss: weights")) return rc;
   }
   unsigned grid = 0;
-  if (a->rows) {
+  if (a->rows || (!a->want_stats && a->dlog_std)) {      // (of no rows at all the gradient of a shared log_std is still to be written)
     BY_TYPE(a->dtype, grid = loss_launch<T>(*a, st));
     if (const int rc = launched("policy loss")) return rc;
   }

@@ -177,7 +177,7 @@ template <class T, int VE> __device__ __forceinline__ void loss_kinds(const RowI
 // what comes before the rows; false: there is nothing to do
 __device__ __forceinline__ bool loss_begin(const agarcl_policy_loss_args &a, LossTotals &t, double *lds) {
   const bool grads = a.dlogits || a.dmean || (a.dlog_std && a.log_std_per_row);
-  t.shared_std = a.mean && !a.log_std_per_row && a.dlog_std;
+  t.shared_std = a.dlog_std && !a.log_std_per_row;
   const float up = a.upstream ? *a.upstream : 1.f;
   if (!a.want_stats) {
     if (t.shared_std && blockIdx.x == 0 && threadIdx.x < 2) ((float *)a.dlog_std)[threadIdx.x] = a.dlog_std_one[threadIdx.x] * up;
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(512) void k_loss_stats(const agarcl_policy_loss_arg
 // wavefront that works on it, so lanes hold several chunks: 65536 rows of 500 bf16 kinds with 64 / 32 / 16 lanes of 1 / 2 / 4 chunks 112 / 56 / 48 us, 300000 of 64 with
 // 8 / 4 / 2 lanes 31 / 25 / 27; 8209 rows of 6144 with 128 threads of 6 chunks 67 us, 256 of 3 76, 1024 of 1 172.  A workgroup of 256 that reads a row twice: 16384 kinds
 // 58 us, where 1024 threads that hold it took 74.
-static unsigned loss_grid(int64_t rows, int64_t per, int64_t most) { const int64_t n = (rows + per - 1) / per; return (unsigned)(n < most ? n : most); }
+static unsigned loss_grid(int64_t rows, int64_t per, int64_t most) { const int64_t n = (rows + per - 1) / per; return (unsigned)(n < 1 ? 1 : n < most ? n : most); }
 template <class T> static unsigned loss_launch(const agarcl_policy_loss_args &a, hipStream_t st) {
   const int64_t V = a.kinds;
   unsigned grid;

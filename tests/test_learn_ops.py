@@ -70,7 +70,8 @@ def memory_bounds(gmax, biggest, steps):
 
 
 SHAPES = [(1, (1,), 1), (1, (5,), 3), (2, (1,), 7), (7, (3,), 5), (8, (2,), 8), (9, (1,), 64), (16, (4,), 32), (17, (33,), 77), (64, (4,), 256), (65, (2, 3), 12), (300, (2,), 4), (1000, (1,), 1),
-          (31, (1000,), 8), (3, (4099,), 5), (2049, (3,), 20), (5000, (2,), 16)]
+          (31, (1000,), 8), (3, (4099,), 5), (2049, (3,), 20), (5000, (2,), 16),
+          (1000, (5,), 13), (700, (1,), 65), (300, (3,), 43), (40, (171,), 3), (9, (1,), 4097), (2, (1,), 65537)]      # (the last: 16-bit columns in pairs, one left over at the head of a workgroup)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
@@ -503,6 +504,10 @@ def test_policy_loss_forms_of_its_arguments(learn):
     zero = both(dict(p, weight=torch.zeros(R, device="cuda")))
     assert all((t == 0).all() for t in zero)
     none = learn.policy_loss(torch.zeros(0, 3, device="cuda", requires_grad=True), torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, device="cuda"), torch.zeros(0, device="cuda"))
+    std = torch.zeros(2, device="cuda", requires_grad=True)
+    moved = learn.policy_loss(torch.zeros(0, 3, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda"), torch.zeros(0, device="cuda"), torch.zeros(0, device="cuda"),
+                              torch.zeros(0, 2, device="cuda"), std, torch.zeros(0, 2, device="cuda"))
+    assert torch.autograd.grad(moved.loss, std)[0].tolist() == [0.0, 0.0]
     assert none.loss.item() == 0 and torch.autograd.grad(none.loss, none.loss)[0].item() == 1
     none.loss.backward()
 

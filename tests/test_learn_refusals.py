@@ -149,7 +149,7 @@ def los(**kw):
 C_BAD = [
     ("agarcl_recurrence", rec(dtype=3)), ("agarcl_recurrence", rec(steps=-1)), ("agarcl_recurrence", rec(rows=1 << 39, width=1 << 39)), ("agarcl_recurrence", rec(x=None)),
     ("agarcl_recurrence", rec(x_stride=5)), ("agarcl_recurrence", rec(gate_stride=-6)), ("agarcl_recurrence", rec(reset=64, reset_stride=1)), ("agarcl_recurrence", rec(h=None)),
-    ("agarcl_recurrence", rec(last=None)), ("agarcl_recurrence", rec(x_stride=1 << 62)),
+    ("agarcl_recurrence", rec(steps=0, rows=1 << 39, width=1 << 39)), ("agarcl_recurrence", rec(last=None)), ("agarcl_recurrence", rec(x_stride=1 << 62)),
     ("agarcl_recurrence_grad", rec(marks=None)), ("agarcl_recurrence_grad", rec(dx=None)), ("agarcl_recurrence_grad", rec(dstate=None)), ("agarcl_recurrence_grad", rec(dh=64, dh_stride=1)),
     ("agarcl_advantages", adv(dtype=-1)), ("agarcl_advantages", adv(gamma=2.0)), ("agarcl_advantages", adv(gamma=float("nan"))), ("agarcl_advantages", adv(returns=None)),
     ("agarcl_advantages", adv(final_value=64, final_stride=2)), ("agarcl_advantages", adv(truncated=64, truncated_stride=1)), ("agarcl_advantages", adv(value_stride=1)),
