@@ -130,9 +130,9 @@ template <class T, int VEC, int ROWS> struct RecurrenceOp {
 
 // E[t] = what reaches h[t-1] = keep f (dh[t] + E[t+1]); G = dh[t] + E[t+1]; dx = (1 - f) G; dgate = G (p - x) f (1 - f).  p, what a step saw of the state, is
 // worked out again from the state kept in front of the segment: in 32 bits, where h itself was rounded, and with fewer bytes than h.  The steps are gone
-// through again from dh, 1 - f and w = (p - x) f (1 - f): three quarters of the registers that P and B of every step would take, and with them a fourth wavefront.
+// through again from dh, 1 - f and w = (p - x) f (1 - f): three quarters of the registers that P and B of every step would take, and with them another wavefront.
 template <class T, int VEC, int ROWS> struct RecurrenceGradOp {
-  static const bool reverse = true; static const int waves = 4;
+  static const bool reverse = true; static const int waves = VEC == 2 ? 3 : 4;      // (pairs: four would spill; 128 x 512 x 64 bf16 16 us with three, 19 with four)
   Rows<const T> x, gate, dh; Resets<VEC, ROWS> resets; Rows<const float> marks; Rows<T> dx, dgate; int64_t steps;
   Raw<T, VEC> xv[SEG], gv[SEG], dn[SEG], dv[SEG]; float mark[VEC]; unsigned cn[ROWS], cut[ROWS]; float q[SEG][VEC], w[SEG][VEC];
   __device__ __forceinline__ void start(int64_t c) { resets.place(c); }

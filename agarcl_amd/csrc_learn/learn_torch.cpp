@@ -21,12 +21,10 @@ using torch::autograd::variable_list;
 
 namespace {
 
-struct Failure { int code; std::string text; };      // -> AgarclError
+struct Failure : std::runtime_error { int code; std::string text; Failure(int c, const std::string &t) : std::runtime_error("agarcl error " + std::to_string(c) + ": " + t), code(c), text(t) {} };      // -> AgarclError
 [[noreturn]] void refuse(const std::string &m) { throw py::value_error(m); }
 void done(int rc) {
-  if (rc == 0) return;
-  if (PyGILState_Check()) throw Failure{rc, agarcl_learn_error()};
-  throw std::runtime_error("agarcl error " + std::to_string(rc) + ": " + agarcl_learn_error());      // (a backward pass in autograd's thread)
+  if (rc != 0) throw Failure(rc, agarcl_learn_error());      // (out of a backward pass it comes as the RuntimeError that it is)
 }
 
 // ---- arguments ------------------------------------------------------------------------------------------------------------------------------
@@ -59,7 +57,8 @@ void on_gpu(const Tensor &t) { if (!t.is_cuda()) refuse("tensors must live on a 
 void *stream_of(const Tensor &t) { return (void *)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 bool capturing(const Tensor &t) {
   hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
-  return hipStreamIsCapturing((hipStream_t)stream_of(t), &s) == hipSuccess && s != hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing((hipStream_t)stream_of(t), &s) != hipSuccess) { (void)hipGetLastError(); return true; }      // (it cannot be asked now: the careful answer)
+  return s != hipStreamCaptureStatusNone;
 }
 int64_t product(at::IntArrayRef s) { int64_t n = 1; for (auto k : s) n *= k; return n; }
 const void *ptr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
@@ -394,8 +393,7 @@ py::tuple policy_loss(py::handle hlogits, py::handle hkind, py::handle hold, py:
 
 PYBIND11_MODULE(_learn, m) {
   m.doc() = "torch tensors in and out of include/agarcl_learn.h; documented in agarcl_amd/learn.py";
-  static py::object error = py::module_::import("agarcl_amd._capi").attr("AgarclError");
-  error.inc_ref();      // (outlives the interpreter's own order of ends)
+  static const py::object &error = *new py::object(py::module_::import("agarcl_amd._capi").attr("AgarclError"));      // (never destroyed: nothing runs after the interpreter)
   py::register_exception_translator([](std::exception_ptr p) {
     try { if (p) std::rethrow_exception(p); }
     catch (const Failure &f) { py::object e = error(f.code, f.text); PyErr_SetObject(error.ptr(), e.ptr()); }
