@@ -268,8 +268,8 @@ class AgarioVectorEnv:
         return obs, {}
 
     def step(self, actions):
-        """actions = (move, kind): move f32 [N, 2] (or [N, num_agents, 2]) in [-1, 1]^2, kind int [N] (or [N, num_agents]) in {0 none, 1 feed,
-        2 split}; CUDA tensors of the right type are used in place, anything else is converted / uploaded.  Everything is enqueued -- on the
+        """actions = (move, kind), or a longer tuple that begins so (learn.sample_actions' result): move f32 [N, 2] (or [N, num_agents, 2]) in
+        [-1, 1]^2, kind int [N] (or [N, num_agents]) in {0 none, 1 feed, 2 split}; CUDA tensors of the right type are used in place, anything else is converted / uploaded.  Everything is enqueued -- on the
         current CUDA stream, or on the sub-batches' own streams ordered against it -- and nothing waits for it.  (Values are not range-checked
         here -- that would need them on the host; the engine clamps nothing either, as the reference's take_action: BaseEnvironment.hpp:162-176.)"""
         assert self._started, "reset() must be called before the first step()"
