@@ -11,6 +11,7 @@
 
 #include <cmath>
 #include <string>
+#include <unordered_set>
 
 #include "../../include/agarcl_learn.h"
 
@@ -29,17 +30,22 @@ void done(int rc) {
 
 // ---- arguments ------------------------------------------------------------------------------------------------------------------------------
 std::string shape_text(at::IntArrayRef s) { std::string t = "("; for (size_t i = 0; i < s.size(); ++i) t += (i ? ", " : "") + std::to_string(s[i]); return t + (s.size() == 1 ? ",)" : ")"); }
+Tensor taken(py::handle h, const char *name) {
+  const Tensor &t = THPVariable_Unpack(h.ptr());
+  if (t._fw_grad(0).defined()) refuse(std::string(name) + " carries a forward-mode gradient: there are none through these operators");      // (better said than lost)
+  return t.resolve_neg();      // (a view that negates when it is read: what stands in memory is not what it says)
+}
 Tensor optional(py::handle h, const char *name) {      // undefined for None
   if (h.is_none()) return {};
   if (!THPVariable_Check(h.ptr())) refuse(std::string(name) + " must be a tensor");
-  return THPVariable_Unpack(h.ptr());
+  return taken(h, name);
 }
 Tensor needed(py::handle h, const char *name) { Tensor t = optional(h, name); if (!t.defined()) refuse(std::string(name) + " must be a tensor"); return t; }
 
 int type_code(at::ScalarType t) { return t == at::kFloat ? AGARCL_F32 : t == at::kBFloat16 ? AGARCL_BF16 : t == at::kHalf ? AGARCL_F16 : -1; }
 Tensor first(py::handle h, const char *name) {      // the tensor that says type and device for the others
   if (!THPVariable_Check(h.ptr()) || type_code(THPVariable_Unpack(h.ptr()).scalar_type()) < 0) refuse(std::string(name) + " must be a float32, bfloat16 or float16 tensor");
-  return THPVariable_Unpack(h.ptr());
+  return taken(h, name);
 }
 void like(const Tensor &t, const char *name, const Tensor &ref, at::ArrayRef<at::ScalarType> types, at::IntArrayRef shape) {
   if (t.device() != ref.device()) refuse(std::string(name) + " must live on " + ref.device().str());
@@ -59,6 +65,21 @@ bool capturing(const Tensor &t) {
   hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing((hipStream_t)stream_of(t), &s) != hipSuccess) { (void)hipGetLastError(); return true; }      // (it cannot be asked now: the careful answer)
   return s != hipStreamCaptureStatusNone;
+}
+// A captured backward pass may not reach a node that another stream made: autograd would have that stream wait for the captured one, which ends the capture and
+// with it the process.  That is so for a leaf whose eager graph still lives, since a leaf has one node for all its graphs.
+void capture_reaches(const Tensor &ref, std::initializer_list<const Tensor *> inputs) {
+  if (!capturing(ref)) return;
+  const auto here = c10::hip::getCurrentHIPStream(ref.get_device()).unwrap().id();
+  std::vector<std::shared_ptr<torch::autograd::Node>> nodes;
+  std::unordered_set<torch::autograd::Node *> seen;
+  const auto look = [&](const std::shared_ptr<torch::autograd::Node> &n) { if (n && seen.insert(n.get()).second) nodes.push_back(n); };
+  for (const Tensor *t : inputs) if (t->defined() && t->requires_grad()) look(t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t));
+  for (size_t i = 0; i < nodes.size(); ++i) {
+    const auto s = nodes[i]->stream();
+    if (s && s->id() != here) refuse("a graph that was made on another stream still holds a node of an input: drop it (its loss, its outputs) before the capture, and capture forward and backward together");
+    for (const auto &e : nodes[i]->next_edges()) { const auto next = e.function; look(next); }
+  }
 }
 int64_t product(at::IntArrayRef s) { int64_t n = 1; for (auto k : s) n *= k; return n; }
 const void *ptr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
@@ -152,6 +173,7 @@ py::tuple gated_recurrence(py::handle hx, py::handle hgate, py::handle hstate, p
   if (reset.defined()) like(reset, "reset", x, FLAGS, x.sizes().slice(0, x.dim() - 1));
   on_gpu(x);
   if (at::GradMode::is_enabled() && (x.requires_grad() || gate.requires_grad() || (state.defined() && state.requires_grad()))) {
+    capture_reaches(x, {&x, &gate, &state});
     auto node = std::shared_ptr<RecurrenceNode>(new RecurrenceNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x, gate, state));
     Remembered r;
@@ -373,6 +395,7 @@ py::tuple policy_loss(py::handle hlogits, py::handle hkind, py::handle hold, py:
   c.need[0] = logits.requires_grad(); c.need[1] = mean.defined() && mean.requires_grad(); c.need[2] = log_std.defined() && log_std.requires_grad();
   Tensor loss;
   if (at::GradMode::is_enabled() && (c.need[0] || c.need[1] || c.need[2])) {
+    capture_reaches(logits, {&logits, &mean, &log_std});
     auto node = std::shared_ptr<PolicyLossNode>(new PolicyLossNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(logits, mean, log_std));
     Tensor std_one;

@@ -19,7 +19,8 @@ Conventions of every function: tensors live on one GPU; a rollout's first axis i
 `value` are float32, bfloat16 or float16, everything that counts, sums or carries a state is float32; flags are bool or uint8.  A wrong argument raises
 ValueError, a failing call AgarclError.  Kernels run on the current stream of the tensors' device, also when that is not the current device.
 Tensors of other strides than a kernel reads are copied first (a step's slice, a row, has to be contiguous; steps and rows may lie apart).  There are no
-gradients of gradients: a backward pass with create_graph raises RuntimeError."""
+gradients of gradients: a backward pass with create_graph raises RuntimeError, a forward-mode gradient ValueError.  Forward and backward pass are captured
+together, with no eager graph of the same leaves alive: autograd would tie its stream to the capture (such a call raises ValueError)."""
 import collections
 
 import torch  # noqa: F401   (its HIP runtime has to be the one that is loaded first)

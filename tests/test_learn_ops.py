@@ -9,6 +9,7 @@ Tolerances, derived, in units of E = 2^-24 (a rounding in 32 bits), before the o
   its gradient: the same bound with M the largest total gradient (Gr = (|dh| + |dlast|) / min(1 - f)); dgate multiplies by (p - x) f (1 - f): at most 2 M / 4, and its error has the
     factors' own, at most (30 + 6 G) E, once more.
 Splitting the steps over threads reorders the same products: each join is a rounding of a product and a sum, at most 2 E more for every halving of the length, 64 E for any length."""
+import gc
 import math
 
 import pytest
@@ -639,6 +640,161 @@ def test_captured_and_replayed(learn, name):
         graphs[1 - i % 2].replay(); graphs[i % 2].replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(both, outs[i % 2])) and all(torch.equal(a, b) for a, b in zip(both, outs[1 - i % 2]))
+
+
+def training(learn, name):
+    """a leaf and a training pass over it that leaves the gradient in leaf.grad: () -> the loss"""
+    if name == "memory":
+        x, gate, state, reset, dh, _ = memory_inputs(20, (6,), 5, torch.float32, 3, "some")
+        leaf = x.requires_grad_()
+        return leaf, lambda: (learn.gated_recurrence(leaf * 2, gate, state, reset)[0] * dh).sum()
+    p = loss_inputs(40, 5, torch.float32, 3, True, False, 0.3, True, True)
+    leaf = p["logits"].detach().requires_grad_()
+    return leaf, lambda: learn.policy_loss(**dict(p, logits=leaf), kl_coef=0.1).loss
+
+
+@pytest.mark.parametrize("name", ["memory", "loss"])
+def test_capture_of_a_backward_pass_beside_an_eager_graph(learn, name):
+    """a leaf's node belongs to the stream of the graph that is alive: the capture refuses the call, and takes it once that graph is gone"""
+    leaf, run = training(learn, name)
+    want = torch.autograd.grad(run(), leaf)[0]
+    alive = run()
+    torch.cuda.synchronize()
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused):
+        dummy = torch.zeros(4, device="cuda")
+        with pytest.raises(ValueError, match="another stream"):
+            run()
+    assert dummy is not None
+    alive.backward()                                   # (the eager graph is as it was)
+    assert torch.equal(leaf.grad, want)
+    del alive
+    gc.collect()
+    leaf.grad = None
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run().backward()
+    for _ in range(3):
+        leaf.grad.fill_(7)                             # (the captured pass writes leaf.grad: it was None when it was captured)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(leaf.grad, want)
+
+
+def test_calls_from_several_threads_at_once(learn):
+    """every thread with a stream of its own, all calling all operators at the same time"""
+    import threading
+    jobs = [everything(learn, seed=s)[0] for s in range(4)]
+    want = [{n: [t.clone() for t in op()] for n, op in job.items()} for job in jobs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                for n, op in jobs[i].items():
+                    got = [t.clone() for t in op()]
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i][n])):
+                        wrong.append((i, n))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_views_that_negate(learn):
+    """the imaginary part of a conjugate lies in memory with the other sign"""
+    base = torch.randn(20, 6, 1, dtype=torch.complex64, generator=rng(1)).cuda()
+    x = base.conj().imag
+    assert x.is_neg()
+    gate = torch.randn(20, 6, 1, generator=rng(2)).cuda()
+    got, want = learn.gated_recurrence(x, gate), learn.gated_recurrence(x.clone(), gate)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- long arrays --------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=IDS[:2])
+def test_steps_that_lie_far_apart(learn, dtype):
+    """20 steps of few columns, 256 MB apart: more than the 32 bits of an offset hold"""
+    T, B, C = 20, 3, 40
+
+    def apart(t):
+        step = (1 << 28) // t.element_size()
+        size = t[0].numel()
+        out = torch.empty((T - 1) * step + size, dtype=t.dtype, device="cuda").as_strided(t.shape, (step,) + t[0].stride())
+        return out.copy_(t)
+
+    x, gate, state, reset, dh, dlast = memory_inputs(T, (B,), C, dtype, 5, "some")
+    leaves = [apart(x).requires_grad_(), gate.clone().requires_grad_(), state.clone().requires_grad_()]
+    h, last = learn.gated_recurrence(*leaves, apart(reset))
+    want = F.recurrence(x, gate, state, reset)
+    hb, gb, gateb = memory_bounds(4.0, 4.0, T)
+    near(h, want[0], hb, "h"); near(last, want[1], hb, "last")
+    got = torch.autograd.grad((h, last), leaves, (apart(dh), dlast))
+    for g, w, bound, name in zip(got, F.recurrence_grads(x, gate, state, reset, dh, dlast), (gb, gateb, gb), ("dx", "dgate", "dstate")):
+        near(g, w, bound, name)
+    r, v, nxt, term, trunc, final = rollout(T, B, dtype, 5, 0.1, 0.1)
+    got = learn.advantages(r, apart(v), nxt, apart(term), trunc, apart(final))
+    want = F.advantages(*(t.cpu() for t in (r, v, nxt, term, trunc, final)), float(torch.tensor(0.99)), float(torch.tensor(0.95)))
+    near(got.advantage, want[0], adv_bound(T, 0.99 * 0.95), "advantage"); near(got.returns, want[1], adv_bound(T, 0.99 * 0.95) + 20 * E, "returns")
+
+
+def test_arrays_beyond_32_bits_of_elements(learn):
+    """more than 2^31 elements and 4 GB in every array of a rollout, an odd number of columns.  Against the formulas in torch's float32: both are off by less than 1e-4"""
+    T, B, C = 9, 53687093, 5                           # 268435465 columns
+    x = torch.empty(T, B, C, dtype=torch.bfloat16, device="cuda").normal_()
+    gate = torch.empty_like(x).normal_()
+    reset = torch.empty(T, B, device="cuda").uniform_() < 0.1
+    h, last = learn.gated_recurrence(x.requires_grad_(), gate.requires_grad_(), None, reset)
+    dlast = torch.ones_like(last)
+    dx, dgate = torch.autograd.grad(last, (x, gate), dlast)
+    off = lambda got, want: ((got.float() - want).abs() - want.abs() * torch.finfo(torch.bfloat16).eps / 2).max().item()      # noqa: E731
+    with torch.no_grad():
+        s, seen = torch.zeros(B, C, device="cuda"), []
+        for t in range(T):
+            f = torch.sigmoid(gate[t].float())
+            seen.append(torch.where(reset[t][:, None], 0, s))
+            s = f * seen[t] + (1 - f) * x[t].float()
+            assert off(h[t], s) < 1e-4, t
+        assert (last - s).abs().max().item() < 1e-4
+        G = dlast
+        for t in reversed(range(T)):
+            f = torch.sigmoid(gate[t].float())
+            assert off(dx[t], (1 - f) * G) < 1e-4 and off(dgate[t], G * (seen[t] - x[t].float()) * f * (1 - f)) < 1e-4, t
+            G = torch.where(reset[t][:, None], 0, f * G)
+    del x, gate, h, last, dx, dgate, s, f, G, seen
+    torch.cuda.empty_cache()
+
+
+def test_logits_beyond_32_bits_of_elements(learn):
+    R, V = 66000, 65543
+    z = torch.empty(R, V, dtype=torch.bfloat16, device="cuda")
+    z.normal_()
+    z.requires_grad_()
+    zeros = torch.zeros(R, device="cuda")
+    weight = zeros.clone()
+    weight[-5:] = 1
+    kind = torch.full((R,), V - 1, dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        a = learn.sample_actions(z)
+        old = a.log_prob
+        assert torch.equal(a.kind[-50:], torch.stack([(row == row.max()).nonzero()[0, 0] for row in z[-50:].float()]).int())
+        lp = torch.log_softmax(d(z[-5:]), -1)
+        near(old[-5:], lp.max(-1).values, lp_err(16.0, V))
+    out = learn.policy_loss(z, kind, torch.cat([zeros[:-5], lp[:, -1].float().cuda()]), torch.ones(R, device="cuda"), weight=weight)
+    (dz,) = torch.autograd.grad(out.loss, z)
+    want = (lp.exp() - torch.eye(V, dtype=torch.float64)[V - 1]) / 5
+    near(dz[-5:], want, 0.2 * 2 * lp_err(16.0, V))      # (the ratio and a probability are each off by as much)
+    assert dz[:-5].count_nonzero().item() == 0
+    del z, dz, out
+    torch.cuda.empty_cache()
 
 
 def test_the_rollout_example_learns_from_its_rollouts(learn):

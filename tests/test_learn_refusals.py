@@ -184,3 +184,12 @@ def test_nothing_to_do_is_no_error(lib):
     assert all(lib.agarcl_recurrence_work(t, b, c) >= 0 for t in (1, 8, 9, 100, 30000) for b in (1, 3, 5000) for c in (1, 2, 7, 256))
     for name, args in (("agarcl_recurrence", rec(rows=0)), ("agarcl_recurrence_grad", rec(width=0)), ("agarcl_advantages", adv(steps=0)), ("agarcl_sample_actions", sam(rows=0))):
         assert getattr(lib, name)(ctypes.byref(args)) == 0, name
+
+
+@pytest.mark.parametrize("name,arg", [("gated_recurrence", "gate"), ("recurrence_step", "x"), ("advantages", "value"), ("policy_loss", "logits"), ("policy_loss", "mean")])
+def test_forward_mode_gradients_are_refused(name, arg):
+    with torch.autograd.forward_ad.dual_level():
+        args = dict(GOOD[name])
+        args[arg] = torch.autograd.forward_ad.make_dual(args[arg].clone(), torch.ones_like(args[arg]))
+        with pytest.raises(ValueError, match=arg + " carries a forward-mode gradient"):
+            getattr(learn, name)(**args)
