@@ -1,37 +1,42 @@
 // learn_recurrence.inl -- the gated recurrence, its gradient, and the advantages, as steps of learn_scan.inl
 
-// flags of a segment: bit i of out[j] for step i and column j
-template <int N> __device__ __forceinline__ void load_flags(unsigned (&out)[N], const uint8_t *flags, int64_t stride, int64_t t0, int n, const int64_t (&row)[N]) {
+// the flags of a segment's steps, as they were loaded (a load that is not looked at yet does not have to be waited for); behind the n there are: 0
+template <int N> struct Flags {
+  uint32_t b[SEG][N];
+  __device__ __forceinline__ void load(const uint8_t *flags, int64_t stride, int64_t t0, int n, const int64_t (&row)[N]) {
+    if (flags && n == SEG) {      // (apart, so that nothing stands between the loads)
 #pragma unroll
-  for (int j = 0; j < N; ++j) out[j] = 0;
-  if (!flags) return;
-  if (n == SEG) {      // (apart, so that nothing stands between the loads)
-    uint8_t b[SEG][N];
+      for (int i = 0; i < SEG; ++i) {
 #pragma unroll
-    for (int i = 0; i < SEG; ++i) {
+        for (int j = 0; j < N; ++j) b[i][j] = flags[(t0 + i) * stride + row[j]];
+      }
+    } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) b[i][j] = flags[(t0 + i) * stride + row[j]];
-    }
+      for (int i = 0; i < SEG; ++i) {
 #pragma unroll
-    for (int i = 0; i < SEG; ++i) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) out[j] |= b[i][j] ? 1u << i : 0u;
-    }
-  } else {
-    for (int i = 0; i < n; ++i) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) out[j] |= flags[(t0 + i) * stride + row[j]] ? 1u << i : 0u;
+        for (int j = 0; j < N; ++j) { b[i][j] = 0; if (flags && i < n) b[i][j] = flags[(t0 + i) * stride + row[j]]; }
+      }
     }
   }
-}
+  __device__ __forceinline__ void bits(unsigned (&out)[N]) const {      // bit i: step i
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      out[j] = 0;
+#pragma unroll
+      for (int i = 0; i < SEG; ++i) out[j] |= b[i][j] ? 1u << i : 0u;
+    }
+  }
+};
 // the steps of a segment; behind the n there are: `none`
 template <class T, int VEC> __device__ __forceinline__ void load_steps(Raw<T, VEC> (&out)[SEG], const Rows<const T> &p, const Place &w, int n, float none) {
-  const uint32_t off = p.offset(w);
+  uint32_t off = p.offset(w);
   uintptr_t at = p.first(w);
   if (n == SEG) {
+    here(off);
 #pragma unroll
     for (int i = 0; i < SEG; ++i, at += p.step()) load_raw<T, VEC>(out[i], device_ptr<const T>(at, off));
   } else {
+    here(off);
 #pragma unroll
     for (int i = 0; i < SEG; ++i, at += p.step()) {
       if (i < n) load_raw<T, VEC>(out[i], device_ptr<const T>(at, off));
@@ -43,9 +48,10 @@ __device__ __forceinline__ int steps_left(int64_t steps, const Place &w) { const
 static __device__ const float kTiny = 1.17549435e-38f;
 // SEG steps of VEC columns; nothing stands between the stores of a whole segment
 template <class T, int VEC> __device__ __forceinline__ void write_steps(const Rows<T> &p, const Place &w, int n, const float (&v)[SEG][VEC]) {
-  const uint32_t off = p.offset(w);
+  uint32_t off = p.offset(w);
   uintptr_t at = p.first(w);
   if (n == SEG) {
+    here(off);
 #pragma unroll
     for (int i = 0; i < SEG; ++i, at += p.step()) store_pack<T, VEC>(device_ptr<T>(at, off), v[i]);
   } else {
@@ -94,16 +100,17 @@ __device__ __forceinline__ Place mark_place(const Place &w) { return Place{w.bas
 template <class T, int VEC, int ROWS> struct RecurrenceOp {
   static const bool reverse = false; static const int waves = 4;
   Rows<const T> x, gate; Resets<VEC, ROWS> resets; Rows<T> h; Rows<float> marks; int64_t steps;      // marks: a row for every segment
-  Raw<T, VEC> xv[SEG], gv[SEG]; unsigned cut[ROWS]; float P[SEG][VEC], B[SEG][VEC];
+  Raw<T, VEC> xv[SEG], gv[SEG]; Flags<ROWS> flags; float P[SEG][VEC], B[SEG][VEC];
   __device__ __forceinline__ void start(int64_t c) { resets.place(c); }
   __device__ __forceinline__ void load(const Place &w) {
     const int n = steps_left(steps, w);
     load_steps<T, VEC>(xv, x, w, n, 0.f);
     load_steps<T, VEC>(gv, gate, w, n, INFINITY);      // (a step that is not there keeps the state)
-    load_flags(cut, resets.reset, resets.rs, w.base + w.t, n, resets.row);
+    flags.load(resets.reset, resets.rs, w.base + w.t, n, resets.row);
   }
   __device__ __forceinline__ void prep(Map<VEC> &m) {
-    float least[ROWS];
+    unsigned cut[ROWS]; float least[ROWS];
+    flags.bits(cut);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) least[j] = kTiny;
 #pragma unroll
@@ -134,7 +141,7 @@ template <class T, int VEC, int ROWS> struct RecurrenceOp {
 template <class T, int VEC, int ROWS> struct RecurrenceGradOp {
   static const bool reverse = true; static const int waves = VEC == 2 ? 3 : 4;      // (pairs: four would spill; 128 x 512 x 64 bf16 16 us with three, 19 with four)
   Rows<const T> x, gate, dh; Resets<VEC, ROWS> resets; Rows<const float> marks; Rows<T> dx, dgate; int64_t steps;
-  Raw<T, VEC> xv[SEG], gv[SEG], dn[SEG], dv[SEG]; float mark[VEC]; unsigned cn[ROWS], cut[ROWS]; float q[SEG][VEC], w[SEG][VEC];
+  Raw<T, VEC> xv[SEG], gv[SEG], dn[SEG], dv[SEG]; float mark[VEC]; Flags<ROWS> flags; unsigned cut[ROWS]; float q[SEG][VEC], w[SEG][VEC];
   __device__ __forceinline__ void start(int64_t c) { resets.place(c); }
   __device__ __forceinline__ void load(const Place &w) {
     const int n = steps_left(steps, w);
@@ -147,12 +154,13 @@ template <class T, int VEC, int ROWS> struct RecurrenceGradOp {
     }
     const Place s = mark_place(w);
     load_floats<VEC>(mark, device_ptr<const float>(marks.first(s), marks.offset(s)));
-    load_flags(cn, resets.reset, resets.rs, w.base + w.t, n, resets.row);
+    flags.load(resets.reset, resets.rs, w.base + w.t, n, resets.row);
   }
   __device__ __forceinline__ void prep(Map<VEC> &m) {
     float s[VEC], f[SEG][VEC], least[ROWS];
+    flags.bits(cut);
 #pragma unroll
-    for (int j = 0; j < ROWS; ++j) { cut[j] = cn[j]; least[j] = kTiny; }
+    for (int j = 0; j < ROWS; ++j) least[j] = kTiny;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) s[j] = mark[j];
 #pragma unroll
@@ -202,7 +210,7 @@ template <class T, int VEC> struct AdvantageOp {
   static const bool reverse = true; static const int waves = 3;
   Rows<const float> reward; Rows<const T> value, final_value; const T *next_value; const uint8_t *terminated, *truncated; int64_t es, us;
   float gamma, gl; Rows<float> advantage, returns; int64_t steps;
-  int64_t row[VEC]; int n; Raw<float, VEC> r[SEG]; Raw<T, VEC> v[SEG], after, f[SEG]; unsigned term[VEC], trunc[VEC]; float P[SEG][VEC], B[SEG][VEC], V[SEG][VEC];
+  int64_t row[VEC]; int n; Raw<float, VEC> r[SEG]; Raw<T, VEC> v[SEG], after, f[SEG]; Flags<VEC> term, trunc; float P[SEG][VEC], B[SEG][VEC], V[SEG][VEC];
   __device__ __forceinline__ void start(int64_t c) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) row[j] = c + j;
@@ -213,8 +221,8 @@ template <class T, int VEC> struct AdvantageOp {
     load_steps<float, VEC>(r, reward, w, n, 0.f);
     load_steps<T, VEC>(v, value, w, n, 0.f);
     load_raw<T, VEC>(after, t0 + n < steps ? device_ptr<const T>(value.first(w) + SEG * value.step(), value.offset(w)) : next_value + row[0]);      // (t0 + n < steps: n = SEG)
-    load_flags(term, terminated, es, t0, n, row);
-    load_flags(trunc, truncated, us, t0, n, row);
+    term.load(terminated, es, t0, n, row);
+    trunc.load(truncated, us, t0, n, row);
     if (final_value.p) load_steps<T, VEC>(f, final_value, w, n, 0.f);
   }
   __device__ __forceinline__ void prep(Map<VEC> &m) {
@@ -223,7 +231,7 @@ template <class T, int VEC> struct AdvantageOp {
       float then = after[j], least = kTiny;
 #pragma unroll
       for (int i = SEG - 1; i >= 0; --i) {
-        const bool there = i < n, end = (term[j] >> i) & 1, off = !end && (trunc[j] >> i) & 1, cut = end || off || (gl == 0.f && there);
+        const bool there = i < n, end = term.b[i][j] != 0, off = !end && trunc.b[i][j] != 0, cut = end || off || (gl == 0.f && there);
         const float now = v[i][j];
         float d = end ? r[i][j] - now : fmaf(gamma, off && final_value.p ? f[i][j] : then, r[i][j]) - now;
         if (off && !final_value.p) d = 0.f;
@@ -248,10 +256,10 @@ template <class T, int VEC> struct AdvantageOp {
   }
 };
 
-template <class Op, int VEC, bool MAPS>
+template <class Op, int VEC, int MODE>
 __global__ __launch_bounds__(256, Op::waves) void k_scan(Op op, const ScanShape sh, const float *start, float *end, float *work) {
   __shared__ ScanLds<VEC> lds;
-  scan_columns<Op, VEC, MAPS>(op, sh, start, end, work, lds);
+  scan_columns<Op, VEC, MODE>(op, sh, start, end, work, lds);
 }
 
 // one step: elementwise, 8 columns of a row's per thread where rows allow it
@@ -321,6 +329,8 @@ static int64_t scan_work(int64_t steps, int64_t columns) {      // floats for an
 
 template <class Op, int VEC> static void scan_launch(const Op &op, const ScanShape &sh, const float *start, float *end, float *work, hipStream_t st) {
   const unsigned gx = (unsigned)(sh.slots < (1 << 20) ? sh.slots : 1 << 20);
-  if (sh.chunks > 1) k_scan<Op, VEC, true><<<dim3(gx, sh.chunks - 1), 256, 0, st>>>(op, sh, start, end, work);
-  k_scan<Op, VEC, false><<<dim3(gx, sh.chunks), 256, 0, st>>>(op, sh, start, end, work);
+  if (sh.chunks > 1) {
+    k_scan<Op, VEC, MAPS><<<dim3(gx, sh.chunks - 1), 256, 0, st>>>(op, sh, start, end, work);
+    k_scan<Op, VEC, CHUNK><<<dim3(gx, sh.chunks), 256, 0, st>>>(op, sh, start, end, work);
+  } else k_scan<Op, VEC, WHOLE><<<dim3(gx, 1), 256, 0, st>>>(op, sh, start, end, work);
 }

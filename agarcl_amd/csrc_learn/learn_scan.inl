@@ -54,6 +54,9 @@ template <class T, int VEC> __device__ __forceinline__ void store_pack(T *p, con
 // device memory at an address that is the same for the wavefront and an offset that is the lane's: the form that loads take without vector arithmetic
 template <class T> __device__ __forceinline__ T *device_ptr(uintptr_t base, uint32_t off) { return (T *)(GLOBAL T *)((GLOBAL char *)base + off); }
 
+// (an offset worked out in another block counts as 64 bits of the lane's, and every access adds the base to them)
+__device__ __forceinline__ void here(uint32_t &off) { asm volatile("" : "+v"(off)); }
+
 template <int VEC> struct Map { float P[VEC], B[VEC]; };
 __device__ __forceinline__ float map_at(float P, float B, float y) { return P == 0.f ? B : fmaf(P, y, B); }
 __device__ __forceinline__ float map_p(float a, float b) { return a == 0.f || b == 0.f ? 0.f : fmaxf(a * b, 1.17549435e-38f); }
@@ -123,8 +126,10 @@ template <class T> struct Rows {      // an array of steps x columns
 };
 
 // Op: load(place) -> registers; prep(Map &): what can be known without the y that enters; write(place, y).  Op::reverse: the last segment is first.
-// work: [2][chunks][columns] maps of the chunks
-template <class Op, int VEC, bool MAPS>
+// work: [2][chunks][columns] maps of the chunks.  MAPS leaves them, CHUNK begins where they lead, WHOLE is a launch without chunks: a kernel of its own, since the
+// registers that the joining of the maps takes would cost it a wavefront per SIMD.
+enum { WHOLE, MAPS, CHUNK };
+template <class Op, int VEC, int MODE>
 __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const float *start, float *end, float *work, ScanLds<VEC> &lds) {
   const ScanLane s = scan_lane(sh.cl_log);
   int parity = 0;
@@ -146,22 +151,9 @@ __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const 
     };
     float y[VEC];
     Map<VEC> run; map_clear(run);
-    if (!MAPS) {
+    if (MODE != MAPS) {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) y[j] = start && there ? start[c0 + j] : 0.f;
-      if (q) {      // the chunks in front: each time lane joins a part of their maps, then all of them
-        const int64_t each = (q + s.tls - 1) / s.tls, lo = s.tl * each, hi = lo + each < q ? lo + each : q;
-        Map<VEC> m, before, all; map_clear(m);
-        for (int64_t c = lo; c < hi; ++c) if (there) {
-          Map<VEC> t;
-          const float *p = work + c * sh.columns + c0, *b = p + sh.chunks * sh.columns;
-          load_floats<VEC>(t.P, p); load_floats<VEC>(t.B, b);
-          map_behind(t, m); m = t;
-        }
-        scan_join(s, m, before, all, lds, parity); parity ^= 1;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = map_at(all.P[j], all.B[j], y[j]);
-      }
     }
     for (int64_t k0 = first - s.tls; k0 < stop; k0 += s.tls) {      // (one turn early: it loads the first segments and does nothing else)
       const bool turn = k0 >= first, on = turn && k0 + s.tl < stop && there;
@@ -169,14 +161,40 @@ __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const 
       map_clear(m);
       if (on) op.prep(m);
       if (k0 + s.tls + s.tl < stop && there) op.load(place(k0 + s.tls));      // (under way while the maps are joined and the steps written)
-      if (!turn) continue;
+      if (!turn) {
+        if (MODE == CHUNK && q) {      // the chunks in front: each time lane joins a part of their maps, then all of them
+          const int64_t each = (q + s.tls - 1) / s.tls, lo = s.tl * each, hi = lo + each < q ? lo + each : q;
+          Map<VEC> f, before, all; map_clear(f);
+          for (int64_t c = lo; c < hi; c += 2) {
+            Map<VEC> t[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              map_clear(t[i]);
+              if (c + i < hi && there) {
+                const float *p = work + (c + i) * sh.columns + c0;
+                load_floats<VEC>(t[i].P, p); load_floats<VEC>(t[i].B, p + sh.chunks * sh.columns);
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) { map_behind(t[i], f); f = t[i]; }
+          }
+          scan_join(s, f, before, all, lds, parity); parity ^= 1;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) y[j] = map_at(all.P[j], all.B[j], y[j]);
+        }
+        if (MODE != MAPS) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) asm volatile("" : "+v"(y[j]));      // (waited for here, or every turn would wait for all the loads that are under way)
+        }
+        continue;
+      }
       float e[VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) e[j] = MAPS ? 0.f : y[j];
-      if (MAPS || s.tls > 1) {
+      for (int j = 0; j < VEC; ++j) e[j] = MODE == MAPS ? 0.f : y[j];
+      if (MODE == MAPS || s.tls > 1) {
         Map<VEC> before, all;
         scan_join(s, m, before, all, lds, parity); parity ^= 1;
-        if (MAPS) { map_behind(all, run); run = all; }
+        if (MODE == MAPS) { map_behind(all, run); run = all; }
         else {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) { e[j] = map_at(before.P[j], before.B[j], y[j]); y[j] = map_at(all.P[j], all.B[j], y[j]); }
@@ -185,10 +203,10 @@ __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const 
 #pragma unroll
         for (int j = 0; j < VEC; ++j) y[j] = map_at(m.P[j], m.B[j], y[j]);
       }
-      if (!MAPS && on) op.write(place(k0), e);
+      if (MODE != MAPS && on) op.write(place(k0), e);
     }
     if (s.tl == 0 && there) {
-      if (MAPS) { store_pack<float, VEC>(work + q * sh.columns + c0, run.P); store_pack<float, VEC>(work + (sh.chunks + q) * sh.columns + c0, run.B); }
+      if (MODE == MAPS) { store_pack<float, VEC>(work + q * sh.columns + c0, run.P); store_pack<float, VEC>(work + (sh.chunks + q) * sh.columns + c0, run.B); }
       else if (end && stop == sh.segments) store_pack<float, VEC>(end + c0, y);
     }
   }
