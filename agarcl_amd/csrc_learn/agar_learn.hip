@@ -78,9 +78,9 @@ extern "C" int agarcl_recurrence(const agarcl_recurrence_args *a) {
     BY_VEC({
       using Op = RecurrenceOp<T, V, R>;
       Op op;
-      op.x = {(uintptr_t)a->x, a->x_stride}; op.gate = {(uintptr_t)a->gate, a->gate_stride}; op.resets.reset = a->reset; op.resets.rs = a->reset_stride;
-      op.resets.width = a->width; op.h = {(uintptr_t)a->h, k}; op.marks = {(uintptr_t)a->marks, k}; op.steps = a->steps;
-      scan_launch<Op, V>(op, scan_shape(a->steps, k, V, reach({a->x_stride, a->gate_stride, k}, sizeof(T))), a->state, a->last, a->work, st);
+      op.x = {(uintptr_t)a->x, a->x_stride}; op.gate = {(uintptr_t)a->gate, a->gate_stride}; op.resets.reset = {(uintptr_t)a->reset, a->reset_stride};
+      op.resets.width = a->width; op.h = {(uintptr_t)a->h, k}; op.marks = {(uintptr_t)a->marks, k}; 
+      scan_launch<Op, V>(op, scan_shape(a->steps, k, V, reach({a->x_stride, a->gate_stride, a->reset ? a->reset_stride : 0, k}, sizeof(T))), a->state, a->last, a->work, st);
     });
   });
   return launched("recurrence");
@@ -101,9 +101,9 @@ extern "C" int agarcl_recurrence_grad(const agarcl_recurrence_args *a) {
       using Op = RecurrenceGradOp<T, V, R>;
       Op op;
       op.x = {(uintptr_t)a->x, a->x_stride}; op.gate = {(uintptr_t)a->gate, a->gate_stride}; op.dh = {(uintptr_t)a->dh, a->dh_stride};
-      op.resets.reset = a->reset; op.resets.rs = a->reset_stride; op.resets.width = a->width; op.marks = {(uintptr_t)a->marks, k}; op.dx = {(uintptr_t)a->dx, k};
-      op.dgate = {(uintptr_t)a->dgate, k}; op.steps = a->steps;
-      scan_launch<Op, V>(op, scan_shape(a->steps, k, V, reach({a->x_stride, a->gate_stride, a->dh ? a->dh_stride : 0, k}, sizeof(T))), a->dlast, a->dstate, a->work, st);
+      op.resets.reset = {(uintptr_t)a->reset, a->reset_stride}; op.resets.width = a->width; op.marks = {(uintptr_t)a->marks, k}; op.dx = {(uintptr_t)a->dx, k};
+      op.dgate = {(uintptr_t)a->dgate, k}; 
+      scan_launch<Op, V>(op, scan_shape(a->steps, k, V, reach({a->x_stride, a->gate_stride, a->dh ? a->dh_stride : 0, a->reset ? a->reset_stride : 0, k}, sizeof(T))), a->dlast, a->dstate, a->work, st);
     });
   });
   return launched("recurrence gradient");
@@ -129,9 +129,10 @@ extern "C" int agarcl_advantages(const agarcl_advantages_args *a) {
   BY_TYPE(a->dtype, {
     AdvantageOp<T, 1> op;
     op.reward = {(uintptr_t)a->reward, a->reward_stride}; op.value = {(uintptr_t)a->value, a->value_stride}; op.final_value = {(uintptr_t)a->final_value, a->final_stride};
-    op.next_value = (const T *)a->next_value; op.terminated = a->terminated; op.truncated = a->truncated; op.es = a->terminated_stride; op.us = a->truncated_stride;
+    op.next_value = {(uintptr_t)a->next_value, 0}; op.terminated = {(uintptr_t)a->terminated, a->terminated_stride};
+    op.truncated = {(uintptr_t)a->truncated, a->truncated_stride};
     op.gamma = a->gamma; op.gl = a->gamma * a->lambda; op.advantage = {(uintptr_t)a->advantage, a->rows}; op.returns = {(uintptr_t)a->returns, a->rows}; op.steps = a->steps;
-    scan_launch<AdvantageOp<T, 1>, 1>(op, scan_shape(a->steps, a->rows, 1, reach({a->reward_stride, a->value_stride, a->final_value ? a->final_stride : 0, a->rows}, 4)), nullptr, nullptr, a->work, st);
+    scan_launch<AdvantageOp<T, 1>, 1>(op, scan_shape(a->steps, a->rows, 1, reach({a->reward_stride, a->value_stride, a->terminated_stride, a->truncated ? a->truncated_stride : 0, a->final_value ? a->final_stride : 0, a->rows}, 4)), nullptr, nullptr, a->work, st);
   });
   return launched("advantages");
 }

@@ -9,7 +9,6 @@
 //
 // A map's P is 0 exactly where a step of it drops what came before (a reset, the end of an episode): joining looks at P and never multiplies what was
 // dropped, so infinities and NaN do not pass.  A product of gates is kept from underflowing to 0 (times 1e-38 is nothing in 32 bits all the same).
-#define GLOBAL __attribute__((address_space(1)))
 
 // VEC neighbouring elements as they were loaded: 16-bit ones stay two to a register
 template <class T, int VEC> struct Raw {
@@ -51,12 +50,6 @@ template <class T, int VEC> __device__ __forceinline__ void store_pack(T *p, con
   for (int j = 0; j < VEC; ++j) k.v[j] = from_f<T>(in[j]);
   *(Pack<T, VEC> *)p = k;
 }
-// device memory at an address that is the same for the wavefront and an offset that is the lane's: the form that loads take without vector arithmetic
-template <class T> __device__ __forceinline__ T *device_ptr(uintptr_t base, uint32_t off) { return (T *)(GLOBAL T *)((GLOBAL char *)base + off); }
-
-// (an offset worked out in another block counts as 64 bits of the lane's, and every access adds the base to them)
-__device__ __forceinline__ void here(uint32_t &off) { asm volatile("" : "+v"(off)); }
-
 template <int VEC> struct Map { float P[VEC], B[VEC]; };
 __device__ __forceinline__ float map_at(float P, float B, float y) { return P == 0.f ? B : fmaf(P, y, B); }
 __device__ __forceinline__ float map_p(float a, float b) { return a == 0.f || b == 0.f ? 0.f : fmaxf(a * b, 1.17549435e-38f); }
@@ -73,7 +66,7 @@ template <int VEC> __device__ __forceinline__ void map_behind(Map<VEC> &m, const
 static const int SEG = AGARCL_MARK_STEPS;
 
 // the shape of a launch: chosen on the host (scan_shape)
-struct ScanShape { int cl_log, chunks; int64_t segments, chunk_segments, columns, groups, slots; };      // slots: groups, up to a multiple of 8
+struct ScanShape { int cl_log, chunks; int64_t steps, segments, chunk_segments, columns, groups, slots; };      // slots: groups, up to a multiple of 8
 
 template <int VEC> struct ScanLds { Map<VEC> total[2][256]; };   // [parity][wavefront (or pair, or all four) x column lane]
 
@@ -115,15 +108,34 @@ template <int VEC> __device__ __forceinline__ void scan_join(const ScanLane &s, 
 }
 
 // Where a thread's segment lies: step t0 of the rollout, `t` steps behind step `base`, which is the same for the workgroup; its columns are `c` behind column
-// `cbase`.  An array's address is then one scalar register pair, a step's stride away from the next step's, and a 32-bit offset of the thread's: no vector
-// arithmetic per load.  The offsets fit: see scan_shape.
-struct Place { int64_t base, cbase; uint32_t t, c; };
-template <class T> struct Rows {      // an array of steps x columns
+// `cbase`.  n: how many of its 8 steps there are (0: the thread has no segment in this turn).
+struct Place { int64_t base, cbase; uint32_t t, c; int n; };
+// An array of steps x columns is read and written through a buffer descriptor per step: the base is the step's (scalar), the offset is the thread's, 32 bits (they
+// fit: see scan_shape).  A step that is not there has an offset behind the descriptor's 2^31 bytes, and an array that is not there has a descriptor of none: such a
+// load gives 0 and such a store is dropped.  So a turn has no branch around its loads and stores, and the compiler can count how many are under way -- with
+// branches it waited for all of them, the stores of the turn before too (20000 x 4 x 64 f32 with its gradient: %s us; with this %s).
+static const uint32_t kGone = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t span(uintptr_t at, bool some) { return __builtin_amdgcn_make_buffer_rsrc((void *)at, 0, some ? kGone : 0, 0x00020000); }
+template <class T> struct Rows {
   uintptr_t p; int64_t stride;
   __device__ __forceinline__ uint32_t offset(const Place &w) const { return (w.t * (uint32_t)stride + w.c) * (uint32_t)sizeof(T); }
   __device__ __forceinline__ uintptr_t first(const Place &w) const { return p + (w.base * stride + w.cbase) * (int64_t)sizeof(T); }      // the same for the workgroup
   __device__ __forceinline__ int64_t step() const { return stride * (int64_t)sizeof(T); }
 };
+__device__ __forceinline__ uint32_t if_there(uint32_t off, bool there) { return there ? off : kGone; }
+template <class T, int VEC> __device__ __forceinline__ void fetch(Raw<T, VEC> &out, __amdgpu_buffer_rsrc_t r, uint32_t off) {
+  if constexpr (VEC * sizeof(T) == 2) out.w[0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+  else if constexpr (VEC * sizeof(T) == 4) out.w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+  else { const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0); out.w[0] = v[0]; out.w[1] = v[1]; }
+}
+template <class T, int VEC> __device__ __forceinline__ void put(__amdgpu_buffer_rsrc_t r, uint32_t off, const float (&in)[VEC]) {
+  Pack<T, VEC> k;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) k.v[j] = from_f<T>(in[j]);
+  if constexpr (VEC * sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, k), r, off, 0, 0);
+  else if constexpr (VEC * sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, k), r, off, 0, 0);
+  else { typedef uint32_t u32x2 __attribute__((ext_vector_type(2))); __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, k), r, off, 0, 0); }
+}
 
 // Op: load(place) -> registers; prep(Map &): what can be known without the y that enters; write(place, y).  Op::reverse: the last segment is first.
 // work: [2][chunks][columns] maps of the chunks.  MAPS leaves them, CHUNK begins where they lead, WHOLE is a launch without chunks: a kernel of its own, since the
@@ -144,10 +156,13 @@ __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const 
     // first, the workgroup begins there, or the offset from its beginning would be below 0)
     if (cbase + VEC > sh.columns) cbase = sh.columns - VEC;
     if (there && c0 + VEC > sh.columns) c0 = sh.columns - VEC;
-    op.start(there ? c0 : 0);
+    op.start(cbase, there ? c0 : cbase);
     // the turn that begins with segment k0 (counted in the scan's order)
     const auto place = [&](int64_t k0) __attribute__((always_inline)) {
-      return Place{(Op::reverse ? sh.segments - s.tls - k0 : k0) * SEG, cbase, (uint32_t)(Op::reverse ? s.tls - 1 - s.tl : s.tl) * SEG, there ? (uint32_t)(c0 - cbase) : 0u};
+      const int64_t low = sh.segments - s.tls - k0, base = Op::reverse ? (low > 0 ? low : 0) : k0, at = Op::reverse ? sh.segments - 1 - k0 - s.tl : k0 + s.tl;
+      const bool on = k0 + s.tl < stop && there;
+      const int64_t left = sh.steps - at * SEG;
+      return Place{base * SEG, cbase, on ? (uint32_t)(at - base) * SEG : 0u, there ? (uint32_t)(c0 - cbase) : 0u, on ? (left < SEG ? (int)left : SEG) : 0};
     };
     float y[VEC];
     Map<VEC> run; map_clear(run);
@@ -155,39 +170,36 @@ __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const 
 #pragma unroll
       for (int j = 0; j < VEC; ++j) y[j] = start && there ? start[c0 + j] : 0.f;
     }
-    for (int64_t k0 = first - s.tls; k0 < stop; k0 += s.tls) {      // (one turn early: it loads the first segments and does nothing else)
-      const bool turn = k0 >= first, on = turn && k0 + s.tl < stop && there;
+    op.load(place(first));
+    if (MODE == CHUNK && q) {      // the chunks in front: each time lane joins a part of their maps, then all of them
+      const int64_t each = (q + s.tls - 1) / s.tls, lo = s.tl * each, hi = lo + each < q ? lo + each : q;
+      Map<VEC> f, before, all; map_clear(f);
+      for (int64_t c = lo; c < hi; c += 2) {
+        Map<VEC> t[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          map_clear(t[i]);
+          if (c + i < hi && there) {
+            const float *p = work + (c + i) * sh.columns + c0;
+            load_floats<VEC>(t[i].P, p); load_floats<VEC>(t[i].B, p + sh.chunks * sh.columns);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { map_behind(t[i], f); f = t[i]; }
+      }
+      scan_join(s, f, before, all, lds, parity); parity ^= 1;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) y[j] = map_at(all.P[j], all.B[j], y[j]);
+    }
+    if (MODE != MAPS) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) asm volatile("" : "+v"(y[j]));      // (waited for here, or every turn would wait for all the loads that are under way)
+    }
+    for (int64_t k0 = first; k0 < stop; k0 += s.tls) {
       Map<VEC> m;
       map_clear(m);
-      if (on) op.prep(m);
-      if (k0 + s.tls + s.tl < stop && there) op.load(place(k0 + s.tls));      // (under way while the maps are joined and the steps written)
-      if (!turn) {
-        if (MODE == CHUNK && q) {      // the chunks in front: each time lane joins a part of their maps, then all of them
-          const int64_t each = (q + s.tls - 1) / s.tls, lo = s.tl * each, hi = lo + each < q ? lo + each : q;
-          Map<VEC> f, before, all; map_clear(f);
-          for (int64_t c = lo; c < hi; c += 2) {
-            Map<VEC> t[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              map_clear(t[i]);
-              if (c + i < hi && there) {
-                const float *p = work + (c + i) * sh.columns + c0;
-                load_floats<VEC>(t[i].P, p); load_floats<VEC>(t[i].B, p + sh.chunks * sh.columns);
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) { map_behind(t[i], f); f = t[i]; }
-          }
-          scan_join(s, f, before, all, lds, parity); parity ^= 1;
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) y[j] = map_at(all.P[j], all.B[j], y[j]);
-        }
-        if (MODE != MAPS) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) asm volatile("" : "+v"(y[j]));      // (waited for here, or every turn would wait for all the loads that are under way)
-        }
-        continue;
-      }
+      if (k0 + s.tl < stop && there) op.prep(m);
+      if (k0 + s.tls < stop) op.load(place(k0 + s.tls));      // (under way while the maps are joined and the steps written)
       float e[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) e[j] = MODE == MAPS ? 0.f : y[j];
@@ -203,7 +215,7 @@ __device__ __forceinline__ void scan_columns(Op &op, const ScanShape &sh, const 
 #pragma unroll
         for (int j = 0; j < VEC; ++j) y[j] = map_at(m.P[j], m.B[j], y[j]);
       }
-      if (MODE != MAPS && on) op.write(place(k0), e);
+      if (MODE != MAPS) op.write(place(k0), e);
     }
     if (s.tl == 0 && there) {
       if (MODE == MAPS) { store_pack<float, VEC>(work + q * sh.columns + c0, run.P); store_pack<float, VEC>(work + (sh.chunks + q) * sh.columns + c0, run.B); }
