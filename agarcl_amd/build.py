@@ -158,7 +158,7 @@ def build_learn_torch(force=False):
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-DTORCH_EXTENSION_NAME=_learn",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-isystem", os.path.join(at, "include"), "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"),
            "-isystem", os.path.join(rocm, "include"), "-I" + sysconfig.get_paths()["include"], src, "-o", out, "-L" + HERE, "-l:libagarcl_hip.so", "-Wl,-rpath,$ORIGIN",
-           "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"]
+           "-L" + os.path.join(at, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"]
     subprocess.check_call(cmd)
     return out
 

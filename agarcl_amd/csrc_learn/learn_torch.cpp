@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
@@ -84,7 +85,14 @@ void capture_reaches(const Tensor &ref, std::initializer_list<const Tensor *> in
 int64_t product(at::IntArrayRef s) { int64_t n = 1; for (auto k : s) n *= k; return n; }
 const void *ptr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void *out(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
-Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor &ref) { return at::empty(shape, at::TensorOptions().dtype(type).device(ref.device())); }
+Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor &ref) { return at::detail::empty_cuda(shape, type, ref.device(), std::nullopt); }      // (at::empty takes a microsecond)
+// a tensor of its own on a part of another's memory, `at` elements behind its beginning: an allocation and its share of the host's time less
+Tensor part(const Tensor &of, int64_t at, at::IntArrayRef shape, at::ScalarType type) {
+  auto t = c10::make_intrusive<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(of.storage()), of.key_set(), c10::scalarTypeToTypeMeta(type));
+  t->set_storage_offset(at);
+  t->set_sizes_contiguous(shape);
+  return Tensor(std::move(t));
+}
 Tensor floats(at::IntArrayRef shape, const Tensor &ref) { return make(shape, at::kFloat, ref); }
 Tensor scratch(int64_t n, const Tensor &ref) { if (n < 0) refuse("sizes out of range"); return n ? floats({n}, ref) : Tensor(); }
 
@@ -277,9 +285,10 @@ py::tuple sample_actions(py::handle hlogits, py::handle hmean, py::handle hstd, 
   a.rows = product(lead); a.kinds = logits.size(-1); a.dtype = type_code(logits.scalar_type()); a.device = logits.get_device();
   a.logits = ptr(z.t); a.logits_stride = z.stride; a.allowed = (const uint8_t *)ptr(k.t); a.allowed_stride = k.stride; a.gumbel = (const float *)ptr(g.t); a.gumbel_stride = g.stride;
   a.mean = ptr(m); a.log_std = ptr(s); a.log_std_per_row = per_row; a.normal = (const float *)ptr(n);
-  const Tensor kind = make(lead, at::kInt, logits), log_prob = floats(lead, logits);
+  const int64_t moves = mean.defined() ? 2 * a.rows : 0;
+  const Tensor all = floats({2 * moves + 2 * a.rows}, logits), kind = part(all, 2 * moves, lead, at::kInt), log_prob = part(all, 2 * moves + a.rows, lead, at::kFloat);
   Tensor raw, move;
-  if (mean.defined()) { raw = floats(mean.sizes(), logits); move = floats(mean.sizes(), logits); }
+  if (mean.defined()) { raw = part(all, 0, mean.sizes(), at::kFloat); move = part(all, moves, mean.sizes(), at::kFloat); }
   a.kind = (int32_t *)out(kind); a.log_prob = (float *)out(log_prob); a.raw = (float *)out(raw); a.move = (float *)out(move); a.stream = stream_of(logits);
   done(agarcl_sample_actions(&a));
   return mean.defined() ? py::make_tuple(move, kind, log_prob, raw) : py::make_tuple(py::none(), kind, log_prob, py::none());
@@ -291,8 +300,9 @@ struct LossCall {
   double low, high, kl, entropy;
   int over, per_row;
   bool need[3];                   // logits, mean, log_std
-  Tensor stats;                   // out
+  Tensor results;                 // out, 16 numbers: the loss's stats from kStats on, its gradients of a shared log_std for an upstream gradient of 1 from kStdOne, the loss at kLoss
 };
+const int kStats = 0, kStdOne = 8, kLoss = 10;
 agarcl_policy_loss_args loss_args(const Tensor &logits, const Tensor &mean, const Tensor &log_std, const LossCall &c, std::vector<Tensor> &kept) {
   const Strided z = rows_of(logits), k = rows_of(c.allowed);
   kept.reserve(16);
@@ -312,16 +322,16 @@ void loss_grads(const LossCall &c, const Tensor &logits, const Tensor &mean, con
   if (c.need[1]) g[1] = make(mean.sizes(), mean.scalar_type(), mean);
   if (c.need[2] && c.per_row) g[2] = make(log_std.sizes(), log_std.scalar_type(), log_std);
 }
-// loss; c.stats; the gradients for an upstream gradient of 1 into what of g is defined, that of a shared log_std into std_one
-Tensor loss_forward(const Tensor &logits, const Tensor &mean, const Tensor &log_std, LossCall &c, const Tensor (&g)[3], const Tensor &std_one) {
+// c.results; the gradients for an upstream gradient of 1 into what of g is defined, that of a shared log_std into c.results
+void loss_forward(const Tensor &logits, const Tensor &mean, const Tensor &log_std, LossCall &c, const Tensor (&g)[3], bool shared_std) {
   std::vector<Tensor> kept;
   agarcl_policy_loss_args a = loss_args(logits, mean, log_std, c, kept);
-  const Tensor loss = floats({}, logits), work = make({agarcl_policy_loss_work()}, at::kDouble, logits);
-  c.stats = floats({8}, logits);
-  a.want_stats = 1; a.loss = (float *)out(loss); a.stats = (float *)out(c.stats); a.work = (double *)out(work);
-  a.dlogits = out(g[0]); a.dmean = out(g[1]); a.dlog_std = std_one.defined() ? out(std_one) : out(g[2]);
+  const Tensor work = make({agarcl_policy_loss_work()}, at::kDouble, logits);
+  c.results = floats({16}, logits);
+  float *r = (float *)out(c.results);
+  a.want_stats = 1; a.loss = r + kLoss; a.stats = r + kStats; a.work = (double *)out(work);
+  a.dlogits = out(g[0]); a.dmean = out(g[1]); a.dlog_std = shared_std ? r + kStdOne : out(g[2]);
   done(agarcl_policy_loss(&a));
-  return loss;
 }
 
 // The gradients for an upstream gradient of 1 -- what loss.backward() brings -- are written by the forward pass, from the registers that hold the logits for the
@@ -329,22 +339,22 @@ Tensor loss_forward(const Tensor &logits, const Tensor &mean, const Tensor &log_
 // gradients out from the logits otherwise.  Every other backward pass (a second one through a kept graph; one that is captured: its replays may bring other
 // upstream gradients) works them out, into tensors of its own.  In float16 a loss is scaled as a rule, so there the forward pass leaves them.
 struct PolicyLossNode : torch::autograd::Node {
-  SavedVariable in_[3], fixed_[7], stats_, std_one_;
+  SavedVariable in_[3], fixed_[7], results_;
   LossCall c;                     // without its tensors
   Tensor ahead_[3];               // the gradients for an upstream gradient of 1
   bool ahead = false;
-  void keep(const Tensor &logits, const Tensor &mean, const Tensor &log_std, LossCall &call, const Tensor &std_one) {
+  void keep(const Tensor &logits, const Tensor &mean, const Tensor &log_std, LossCall &call) {
     const Tensor *in[3] = {&logits, &mean, &log_std}, *fixed[7] = {&call.kind, &call.old, &call.adv, &call.move, &call.ref, &call.allowed, &call.weight};
     for (int i = 0; i < 3; ++i) in_[i] = SavedVariable(*in[i], false);
     for (int i = 0; i < 7; ++i) fixed_[i] = SavedVariable(*fixed[i], false);
-    stats_ = SavedVariable(call.stats, false); std_one_ = SavedVariable(std_one, false);
+    results_ = SavedVariable(call.results, false);
     c = LossCall{{}, {}, {}, {}, {}, {}, {}, call.low, call.high, call.kl, call.entropy, call.over, call.per_row, {call.need[0], call.need[1], call.need[2]}, {}};
   }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     for (auto &s : in_) s.reset_data();
     for (auto &s : fixed_) s.reset_data();
-    stats_.reset_data(); std_one_.reset_data();
+    results_.reset_data();
     for (auto &t : ahead_) t.reset();
     ahead = false;
   }
@@ -352,9 +362,9 @@ struct PolicyLossNode : torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     no_second_gradient();
     if (!up[0].defined()) return variable_list(3);
-    const Tensor logits = in_[0].unpack(), mean = in_[1].unpack(), log_std = in_[2].unpack(), stats = stats_.unpack(), std_one = std_one_.unpack();
+    const Tensor logits = in_[0].unpack(), mean = in_[1].unpack(), log_std = in_[2].unpack(), results = results_.unpack();
     LossCall now{fixed_[0].unpack(), fixed_[1].unpack(), fixed_[2].unpack(), fixed_[3].unpack(), fixed_[4].unpack(), fixed_[5].unpack(), fixed_[6].unpack(), c.low, c.high, c.kl, c.entropy,
-                 c.over, c.per_row, {c.need[0], c.need[1], c.need[2]}, stats};
+                 c.over, c.per_row, {c.need[0], c.need[1], c.need[2]}, results};
     std::vector<Tensor> kept;
     agarcl_policy_loss_args a = loss_args(logits, mean, log_std, now, kept);
     const Tensor upstream = up[0].to(at::kFloat).contiguous();
@@ -364,8 +374,8 @@ struct PolicyLossNode : torch::autograd::Node {
       for (int i = 0; i < 3; ++i) g[i] = std::move(ahead_[i]);
     } else loss_grads(now, logits, mean, log_std, g);
     if (c.need[2] && !c.per_row) g[2] = floats({2}, logits);
-    a.upstream = (const float *)ptr(upstream); a.weight_sum = (const float *)ptr(stats) + 4;
-    a.dlogits = out(g[0]); a.dmean = out(g[1]); a.dlog_std = out(g[2]); a.dlog_std_one = (const float *)ptr(std_one);
+    a.upstream = (const float *)ptr(upstream); a.weight_sum = (const float *)ptr(results) + kStats + 4;
+    a.dlogits = out(g[0]); a.dmean = out(g[1]); a.dlog_std = out(g[2]); a.dlog_std_one = (const float *)ptr(results) + kStdOne;
     done(agarcl_policy_loss(&a));
     return {g[0], g[1], g[2]};
   }
@@ -393,23 +403,23 @@ py::tuple policy_loss(py::handle hlogits, py::handle hkind, py::handle hold, py:
   if (c.weight.defined() && c.weight.scalar_type() != at::kFloat) c.weight = c.weight.to(at::kFloat);
   if (c.kind.scalar_type() != at::kInt) c.kind = c.kind.clamp(-1, logits.size(-1)).to(at::kInt);      // (what 32 bits cannot hold is outside all the same)
   c.need[0] = logits.requires_grad(); c.need[1] = mean.defined() && mean.requires_grad(); c.need[2] = log_std.defined() && log_std.requires_grad();
-  Tensor loss;
+  std::shared_ptr<PolicyLossNode> node;
   if (at::GradMode::is_enabled() && (c.need[0] || c.need[1] || c.need[2])) {
     capture_reaches(logits, {&logits, &mean, &log_std});
-    auto node = std::shared_ptr<PolicyLossNode>(new PolicyLossNode(), torch::autograd::deleteNode);
+    node = std::shared_ptr<PolicyLossNode>(new PolicyLossNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(logits, mean, log_std));
-    Tensor std_one;
     {
       at::NoGradGuard off;
       node->ahead = logits.scalar_type() != at::kHalf && !capturing(logits);
       if (node->ahead) loss_grads(c, logits, mean, log_std, node->ahead_);
-      if (c.need[2] && !c.per_row) std_one = floats({2}, logits);
-      loss = loss_forward(logits, mean, log_std, c, node->ahead_, std_one);
+      loss_forward(logits, mean, log_std, c, node->ahead_, c.need[2] && !c.per_row);
     }
-    node->keep(logits, mean, log_std, c, std_one);
-    torch::autograd::set_history(loss, node);
-  } else loss = loss_forward(logits, mean, log_std, c, {}, {});
-  return py::make_tuple(loss, c.stats.select(0, 0), c.stats.select(0, 1), c.stats.select(0, 2), c.stats.select(0, 3));
+    node->keep(logits, mean, log_std, c);
+  } else loss_forward(logits, mean, log_std, c, {}, false);
+  const auto number = [&](int i) { return part(c.results, i, {}, at::kFloat); };
+  const Tensor loss = number(kLoss);
+  if (node) torch::autograd::set_history(loss, node);
+  return py::make_tuple(loss, number(kStats), number(kStats + 1), number(kStats + 2), number(kStats + 3));
 }
 
 }  // namespace
