@@ -72,7 +72,8 @@ def memory_bounds(gmax, biggest, steps):
 
 SHAPES = [(1, (1,), 1), (1, (5,), 3), (2, (1,), 7), (7, (3,), 5), (8, (2,), 8), (9, (1,), 64), (16, (4,), 32), (17, (33,), 77), (64, (4,), 256), (65, (2, 3), 12), (300, (2,), 4), (1000, (1,), 1),
           (31, (1000,), 8), (3, (4099,), 5), (2049, (3,), 20), (5000, (2,), 16),
-          (1000, (5,), 13), (700, (1,), 65), (300, (3,), 43), (40, (171,), 3), (9, (1,), 4097), (2, (1,), 65537)]      # (the last: 16-bit columns in pairs, one left over at the head of a workgroup)
+          (1000, (5,), 13), (700, (1,), 65), (300, (3,), 43), (40, (171,), 3), (9, (1,), 4097), (2, (1,), 65537),      # (the last: 16-bit columns in pairs, one left over at the head of a workgroup)
+          (1100, (1031,), 1), (24, (33000,), 4), (1500, (70,), 1), (2040, (9,), 5), (600, (1001,), 2)]      # (a shape of launch each)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
@@ -234,7 +235,7 @@ def adv_bound(T, gl):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
-@pytest.mark.parametrize("T,B", [(1, 1), (1, 70), (2, 3), (7, 5), (8, 8), (9, 64), (32, 64), (33, 257), (129, 16), (300, 4), (257, 1030), (2000, 1), (9001, 3)])
+@pytest.mark.parametrize("T,B", [(1, 1), (1, 70), (2, 3), (7, 5), (8, 8), (9, 64), (32, 64), (33, 257), (129, 16), (300, 4), (257, 1030), (2000, 1), (9001, 3), (1100, 1031), (520, 4100), (2040, 45), (600, 2003)])
 def test_advantages(learn, T, B, dtype):
     for seed, (p_term, p_trunc, with_trunc, with_final, gamma, lam) in enumerate([(0.0, 0, False, False, 0.99, 0.95), (0.1, 0.1, True, False, 0.99, 0.95), (0.1, 0.1, True, True, 0.999, 1.0),
                                                                                   (1.1, 0.5, True, True, 0.9, 0.9), (0.05, 1.1, True, False, 0.9, 0.9), (0.1, 0.1, True, True, 0.9, 0.0),
