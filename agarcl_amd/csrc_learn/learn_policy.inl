@@ -2,11 +2,12 @@
 //
 // Both are one pass over the logits: a row is in registers (or, beyond 8192 kinds, read twice) while its maximum, the sum s of e^(z - max) and
 // u = sum of e^(z - max) (z - max) are taken; log s and u / s give the log-probabilities and the entropy, and the gradient is written from the same registers:
-// reading the logits once and writing their gradient once is all the memory traffic there has to be (8209 rows of 6144 bf16, masked, with all gradients: 252 MB in 64 us,
-// 3.95 TB/s, where a large copy reaches 4.76: two exps and a dozen other instructions per kind stand beside it).  Up to 8 kinds a row is one thread's, up to 2048
+// reading the logits once and writing their gradient once is all the memory traffic there has to be (8209 rows of 6144 bf16, masked, with all gradients: 252 MB in 61 us,
+// 4.1 TB/s, where a large copy reaches 4.76: two exps and a dozen other instructions per kind stand beside it).  Up to 8 kinds a row is one thread's, up to 2048
 // a group of 1 to 64 lanes', beyond that a workgroup's.
 
-static const int kLossBlocks = 2048, kWeightBlocks = 256;
+static const int kUnits = 256;      // compute units of an MI355X
+static const int kLossBlocks = 2560, kWeightBlocks = 256;
 static const int64_t kLossWork = 8 * kLossBlocks + kWeightBlocks;
 static const float kHalfLog2Pi = 0.91893853320467274f, kHalfLog2PiE = 1.4189385332046727f;
 
@@ -292,9 +293,9 @@ template <class T, int CHUNKS> struct Share {
   }
 };
 
-// CHUNKS x 8 << g_log kinds, a group of 1 << g_log lanes per row
-template <class T, int CHUNKS>
-__global__ __launch_bounds__(256) void k_loss_lanes(const agarcl_policy_loss_args a, const int g_log) {
+// CHUNKS x 8 << g_log kinds, a group of 1 << g_log lanes per row; W wavefronts per SIMD
+template <class T, int CHUNKS, int W>
+__global__ __launch_bounds__(256, W) void k_loss_lanes(const agarcl_policy_loss_args a, const int g_log) {
   __shared__ double lds[32];
   LossTotals t;
   if (!loss_begin(a, t, lds)) return;
@@ -339,8 +340,8 @@ template <int NT> __device__ __forceinline__ RowSums join_waves(const RowSums &m
 }
 
 // NT x 8 x CHUNKS kinds in registers, a workgroup per row; CHUNKS = 0: any number, read twice
-template <class T, int NT, int CHUNKS>
-__global__ __launch_bounds__(NT) void k_loss_block(const agarcl_policy_loss_args a) {
+template <class T, int NT, int CHUNKS, int W>
+__global__ __launch_bounds__(NT, W) void k_loss_block(const agarcl_policy_loss_args a) {
   __shared__ double lds[NT / 64 * 8];
   __shared__ float wl[2][NT / 64][4];
   LossTotals t;
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(NT) void k_loss_block(const agarcl_policy_loss_args
 }
 
 // the workgroups' sums in a fixed order: the same inputs give the same bits.  One wavefront per sum, so that its loads are all under way at once (a wavefront that
-// took all seven in turn needed 6.7 us for 2048 workgroups)
+// took all seven in turn needed 6.7 us for 2048 workgroups, this 4)
 __global__ __launch_bounds__(512) void k_loss_stats(const agarcl_policy_loss_args a, int blocks) {
   __shared__ double sums[8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -419,35 +420,47 @@ __global__ __launch_bounds__(512) void k_loss_stats(const agarcl_policy_loss_arg
 }
 
 // How many kinds call for which kernel.  What a row needs besides its kinds (a logarithm, exponentials, the sums over its lanes) is a few hundred instructions of every
-// wavefront that works on it, so lanes hold several chunks: 65536 rows of 500 bf16 kinds with 64 / 32 / 16 lanes of 1 / 2 / 4 chunks 112 / 56 / 48 us, 300000 of 64 with
-// 8 / 4 / 2 lanes 31 / 25 / 27; 8209 rows of 6144 with 128 threads of 6 chunks 67 us, 256 of 3 76, 1024 of 1 172.  A workgroup of 256 that reads a row twice: 16384 kinds
-// 58 us, where 1024 threads that hold it took 74.
+// wavefront that works on it, so lanes hold several chunks: 65536 rows of 500 bf16 kinds with 64 / 32 lanes of 1 / 2 chunks 112 / 56 us.  As many workgroups as are
+// resident at once, for the most wavefronts per SIMD whose registers hold the chunks: those that wait for a place come late and alone.  40 to 50 million kinds, us:
+//   lanes       2 chunks or, of 16-bit kinds, 3 where their lanes are filled better; bf16 with a mask / f32 of 350 kinds 3 chunks 56 / 45, 2 chunks more than 62 / 44;
+//               of 1000 kinds 2 chunks 55 / 43, 4 chunks 56 / 44, with 4 workgroups per unit instead of as many as are resident 68 / 43; of 2048 4 chunks 55 / 43
+//   workgroups  4000 kinds 128 x 4 chunks 66 / 52, 256 x 2 71 / 51; 6144 kinds 256 x 3 64 / 49, 128 x 6 68 / 54; 8000 kinds 256 x 4 66 / 53, 128 x 8 75 / 61.
+//               Twice as many workgroups as are resident: 6144 kinds 68 instead of 64, f32 71 instead of 49
+//   beyond      a workgroup of 256 reads a row twice: 9000 kinds 79 / 62; 1024 threads that hold a row of 16384 took 74 us where this took 58
 static unsigned loss_grid(int64_t rows, int64_t per, int64_t most) { const int64_t n = (rows + per - 1) / per; return (unsigned)(n < 1 ? 1 : n < most ? n : most); }
+template <class T, int CHUNKS, int W> static unsigned lanes_launch(const agarcl_policy_loss_args &a, hipStream_t st) {
+  int g_log = 0;
+  while ((CHUNKS * 8 << g_log) < a.kinds) ++g_log;
+  const unsigned grid = loss_grid(a.rows, 256 >> g_log, kUnits * W);
+  k_loss_lanes<T, CHUNKS, W><<<dim3(grid), 256, 0, st>>>(a, g_log);
+  return grid;
+}
+template <class T, int NT, int CHUNKS, int W> static unsigned block_launch(const agarcl_policy_loss_args &a, hipStream_t st) {
+  static_assert(kUnits * W * 256 / NT <= kLossBlocks, "work holds the sums of kLossBlocks workgroups");
+  const unsigned grid = loss_grid(a.rows, 1, kUnits * W * 256 / NT);
+  k_loss_block<T, NT, CHUNKS, W><<<dim3(grid), NT, 0, st>>>(a);
+  return grid;
+}
 template <class T> static unsigned loss_launch(const agarcl_policy_loss_args &a, hipStream_t st) {
   const int64_t V = a.kinds;
-  unsigned grid;
+  constexpr bool H = sizeof(T) == 2;
+  const auto room = [&](int64_t chunks) { int64_t n = chunks * 8; while (n < V) n *= 2; return n; };      // the kinds that the lanes of a row hold
   if (V <= 8) {
-    grid = loss_grid(a.rows, 256, kLossBlocks / 2);
+    const unsigned grid = loss_grid(a.rows, 256, kUnits * 4);
     switch ((int)V) {
 #define ONE(n) case n: k_loss_thread<T, n><<<dim3(grid), 256, 0, st>>>(a); break;
       ONE(1) ONE(2) ONE(3) ONE(4) ONE(5) ONE(6) ONE(7) ONE(8)
 #undef ONE
     }
-  } else if (V <= 2048) {
-    const int chunks = V <= 128 ? 2 : 4;
-    int g_log = 0;
-    while ((chunks * 8 << g_log) < V) ++g_log;
-    grid = loss_grid(a.rows, 256 >> g_log, kLossBlocks / 2);
-    if (chunks == 2) k_loss_lanes<T, 2><<<dim3(grid), 256, 0, st>>>(a, g_log);
-    else k_loss_lanes<T, 4><<<dim3(grid), 256, 0, st>>>(a, g_log);
-  } else {
-    grid = loss_grid(a.rows, 1, kLossBlocks);
-    if (V <= 128 * 8 * 4) k_loss_block<T, 128, 4><<<dim3(grid), 128, 0, st>>>(a);
-    else if (V <= 128 * 8 * 6) k_loss_block<T, 128, 6><<<dim3(grid), 128, 0, st>>>(a);
-    else if (V <= 128 * 8 * 8) k_loss_block<T, 128, 8><<<dim3(grid), 128, 0, st>>>(a);
-    else k_loss_block<T, 256, 0><<<dim3(grid), 256, 0, st>>>(a);
+    return grid;
   }
-  return grid;
+  if (V <= 1536 && (V > 1024 || (H && room(3) < room(2)))) return lanes_launch<T, 3, H ? 6 : 5>(a, st);
+  if (V <= 1024) return lanes_launch<T, 2, H ? 7 : 5>(a, st);
+  if (V <= 2048) return lanes_launch<T, 4, H ? 5 : 4>(a, st);
+  if (V <= 128 * 8 * 4) return block_launch<T, 128, 4, H ? 5 : 4>(a, st);
+  if (V <= 256 * 8 * 3) return block_launch<T, 256, 3, H ? 6 : 5>(a, st);
+  if (V <= 256 * 8 * 4) return block_launch<T, 256, 4, H ? 5 : 4>(a, st);
+  return block_launch<T, 256, 0, 7>(a, st);
 }
 
 // Sampling: the same pass with the largest score beside the sums.  65536 rows of 24 bf16 kinds, masked, with gumbel 5.2 us (2.2 TB/s: latency); 4096 of 3 with a move 3.1,

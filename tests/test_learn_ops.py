@@ -324,7 +324,7 @@ def policy_inputs(R, V, dtype, seed, move=True, per_row=False, mask=0.0, junk=Tr
 
 
 SIZES = [(1, 1), (1, 3), (5, 2), (70, 3), (257, 4), (33, 5), (64, 8), (31, 9), (130, 24), (9, 63), (9, 64), (9, 65), (17, 129), (6, 511), (6, 513), (5, 1000), (4, 2049), (3, 5001), (3, 9000),
-         (3, 33000), (2, 70001)]
+         (3, 33000), (2, 70001), (4, 1300), (4, 1800), (3, 7001)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
@@ -476,8 +476,8 @@ def test_policy_loss_and_its_gradients(learn, R, V, dtype):
 
 
 def test_policy_loss_over_many_rows(learn):
-    for V, dtype in ((3, torch.float32), (24, torch.bfloat16)):
-        p = loss_inputs(20011, V, dtype, 8, True, False, 0.2, True, True)
+    for R, V, dtype in ((20011, 3, torch.float32), (20011, 24, torch.bfloat16), (15001, 511, torch.bfloat16), (1601, 5001, torch.bfloat16), (1301, 8001, torch.float32)):
+        p = loss_inputs(R, V, dtype, 8, True, False, 0.2, True, True)
         check_loss(learn, p, V, dtype, dict(clip=(0.2, 0.3), kl_coef=0.1, entropy_coef=0.01))
 
 
