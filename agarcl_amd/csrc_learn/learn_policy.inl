@@ -131,7 +131,9 @@ template <class T> __device__ __forceinline__ LossRow loss_row(const agarcl_poli
   const float share = in.w * t.inv, ce = a.entropy_coef;
   o.sg = share * g; o.c1 = share * ce * rs; o.c0 = (ce != 0.f ? share * ce * (hcat - log_s) - o.sg : -o.sg) * rs;
   if (leader) {
-    const float low = A == 0.f ? 0.f : fminf(ratio * A, fminf(fmaxf(ratio, lowest), high) * A), w = in.w;
+    // (the minimum and maximum that pass a NaN on, as in `below`: the others would make a clipped ratio of it.  And an infinite ratio of no advantage is nothing)
+    const float limited = __builtin_elementwise_minimum(__builtin_elementwise_maximum(ratio, lowest), high), w = in.w;
+    const float low = A == 0.f && ratio == ratio ? 0.f : __builtin_elementwise_minimum(ratio * A, limited * A);
     acc[0] += w;
     if (in.counts) {
       acc[1] += w * low; acc[2] += w * kl; acc[3] += w * ent; acc[4] += clipped ? w : 0.f;

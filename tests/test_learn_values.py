@@ -1,0 +1,72 @@
+"""agarcl_amd.learn on the GPU where an error would hide: policies that are NaN, small forget factors, upstream gradients that are not plain numbers in memory, what becomes
+of the outputs afterwards.  Tolerances in units of E = 2^-24, on top of those of test_learn_ops.py."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ["f32", "bf16", "f16"]
+KINDS = [1, 3, 8, 9, 63, 500, 1000, 1300, 1800, 2049, 5001, 7001, 9000]      # every kernel of the loss and of sampling
+nan, inf = float("nan"), float("inf")
+
+
+@pytest.fixture(scope="module")
+def learn(hip_engine_cls):
+    import os
+    from agarcl_amd import build
+    if not os.path.exists(build.learn_torch_out()):
+        build.build_learn_torch()
+    from agarcl_amd import learn as module
+    return module
+
+
+def rng(seed):
+    g = torch.Generator()
+    g.manual_seed(seed)
+    return g
+
+
+# ---- policies that are NaN ------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("V", KINDS)
+def test_a_nan_logit_shows_in_the_loss(learn, V, dtype):
+    R = 12
+    for A in (1.5, -1.5, 0.0):
+        for at in {V // 2, V - 1}:                           # the row's own kind, and another one
+            z = torch.randn(R, V, generator=rng(V)).to("cuda", dtype)
+            kind = torch.full((R,), V // 2, dtype=torch.int32, device="cuda")
+            old, adv = torch.full((R,), -1.0, device="cuda"), torch.ones(R, device="cuda")
+            z[7, at], adv[7] = nan, A
+            leaf = z.clone().requires_grad_()
+            out = learn.policy_loss(leaf, kind, old, adv)
+            (dz,) = torch.autograd.grad(out.loss, leaf)
+            assert out.loss.isnan() and out.surrogate.isnan() and out.kl.isnan() and out.entropy.isnan(), (A, at)
+            assert torch.isfinite(torch.cat((dz[:7], dz[8:]))).all()
+            weight = torch.ones(R, device="cuda")
+            weight[7] = 0                                    # a row that is left out is not looked at
+            assert all(torch.isfinite(t) for t in learn.policy_loss(z, kind, old, adv, weight=weight))
+            allowed = torch.ones(R, V, dtype=torch.bool, device="cuda")
+            allowed[7, at] = False                           # nor is a kind that is not allowed
+            assert all(torch.isfinite(t) for t in learn.policy_loss(z, kind, old, adv, allowed=allowed))
+
+
+@pytest.mark.parametrize("what", ["mean", "log_std", "move", "old_log_prob"])
+def test_any_nan_shows_in_the_loss(learn, what):
+    for A in (2.0, -2.0, 0.0):
+        p = dict(logits=torch.zeros(9, 3), kind=torch.zeros(9, dtype=torch.int32), old_log_prob=torch.full((9,), -3.0), advantage=torch.full((9,), A), mean=torch.zeros(9, 2),
+                 log_std=torch.zeros(9, 2), move=torch.zeros(9, 2))
+        p[what][4 if p[what].dim() == 1 else (4, 1)] = nan
+        out = learn.policy_loss(**{k: t.cuda() for k, t in p.items()})
+        assert out.loss.isnan() and out.surrogate.isnan(), A
+
+
+def test_infinite_ratios_are_still_clipped(learn):
+    """a ratio that overflows: clipped where that is the lesser, and nothing of it with an advantage of 0"""
+    z, kind, old = torch.zeros(1, 1, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full((1,), -200.0, device="cuda")
+    for A, want in ((1.0, -1.2), (-1.0, inf), (0.0, 0.0)):
+        leaf = z.clone().requires_grad_()
+        out = learn.policy_loss(leaf, kind, old, torch.full((1,), A, device="cuda"))
+        assert out.loss.item() == torch.tensor(want).item()
