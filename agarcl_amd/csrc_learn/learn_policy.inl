@@ -500,8 +500,8 @@ template <class T> __device__ __forceinline__ void pick_write(const agarcl_sampl
     for (int d = 0; d < 2; ++d) {
       const float ls = log_std_at<T>(a.log_std, a.log_std_per_row, row, d), n = a.normal ? a.normal[2 * row + d] : 0.f;
       raw[d] = fmaf(expf(ls), n, to_f(((const T *)a.mean)[2 * row + d]));
-      move[d] = fminf(fmaxf(raw[d], -1.f), 1.f);
-      lp -= 0.5f * n * n + ls + kHalfLog2Pi;
+      move[d] = __builtin_elementwise_minimum(__builtin_elementwise_maximum(raw[d], -1.f), 1.f);      // (a NaN stays one, and shows in the log-probability, where a NaN mean would not)
+      lp -= raw[d] == raw[d] ? 0.5f * n * n + ls + kHalfLog2Pi : raw[d];
     }
     store_pack<float, 2>(a.raw + 2 * row, raw); store_pack<float, 2>(a.move + 2 * row, move);
   }

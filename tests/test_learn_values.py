@@ -70,3 +70,18 @@ def test_infinite_ratios_are_still_clipped(learn):
         leaf = z.clone().requires_grad_()
         out = learn.policy_loss(leaf, kind, old, torch.full((1,), A, device="cuda"))
         assert out.loss.item() == torch.tensor(want).item()
+
+
+@pytest.mark.parametrize("V", [3, 24, 5000])
+@pytest.mark.parametrize("what", ["mean", "log_std", "normal"])
+def test_a_nan_move_is_not_a_move(learn, V, what):
+    p = dict(logits=torch.randn(9, V, generator=rng(V)), mean=torch.randn(9, 2, generator=rng(1)) * 2, log_std=torch.zeros(9, 2), normal=torch.randn(9, 2, generator=rng(2)))
+    good = learn.sample_actions(**{k: t.cuda() for k, t in p.items()})
+    p[what][4, 1] = nan
+    a = learn.sample_actions(**{k: t.cuda() for k, t in p.items()})
+    assert a.raw[4, 1].isnan() and a.move[4, 1].isnan() and a.log_prob[4].isnan()
+    assert torch.equal(a.move[4, 0], good.move[4, 0]) and torch.equal(a.kind, good.kind)
+    rest = [i for i in range(9) if i != 4]
+    assert all(torch.equal(s[rest], t[rest]) for s, t in zip(a, good))
+    p["mean"], p["log_std"], p["normal"] = torch.tensor([[inf, -inf]]).repeat(9, 1), torch.zeros(9, 2), torch.zeros(9, 2)
+    assert learn.sample_actions(**{k: t.cuda() for k, t in p.items()}).move.tolist() == [[1.0, -1.0]] * 9
