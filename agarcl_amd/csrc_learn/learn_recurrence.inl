@@ -132,12 +132,13 @@ template <class T, int VEC, int ROWS> struct RecurrenceOp {
 
 // E[t] = what reaches h[t-1] = keep f (dh[t] + E[t+1]); G = dh[t] + E[t+1]; dx = (1 - f) G; dgate = G (p - x) f (1 - f).  p, what a step saw of the state, is
 // worked out again from the state kept in front of the segment: in 32 bits, where h itself was rounded, and with fewer bytes than h.  The steps are gone
-// through again from dh, 1 - f and w = (p - x) f (1 - f): three quarters of the registers that P and B of every step would take, and with them another wavefront.
+// through again from dh, the lesser of f and 1 - f (sigmoid_again makes both of it) and w = (p - x) f (1 - f): three quarters of the registers that P and B of every step
+// would take, and with them another wavefront.
 // Bound by HBM as the forward pass is: 256 x 4096 x 64 bf16 147 us (4.8 TB/s), x 32 f32 138 us (5.0); 20000 x 4 x 64 f32 41 us in two launches.
 template <class T, int VEC, int ROWS> struct RecurrenceGradOp {
   static const bool reverse = true; static const int waves = VEC == 2 ? 3 : 4;      // (pairs: with the registers of four, half of the types spill)
   Rows<const T> x, gate, dh; Resets<VEC, ROWS> resets; Rows<const float> marks; Rows<T> dx, dgate;
-  Raw<T, VEC> xv[SEG], gv[SEG], dn[SEG], dv[SEG]; Raw<float, VEC> mark; int n; Flags<ROWS> flags; unsigned cut[ROWS]; float q[SEG][VEC], w[SEG][VEC];
+  Raw<T, VEC> xv[SEG], gv[SEG], dn[SEG], dv[SEG]; Raw<float, VEC> mark; int n; Flags<ROWS> flags; unsigned cut[ROWS]; float s[SEG][VEC], w[SEG][VEC];
   __device__ __forceinline__ void start(int64_t cbase, int64_t c) { resets.place(cbase, c); }
   __device__ __forceinline__ void load(const Place &w) {
     n = w.n;
@@ -149,22 +150,22 @@ template <class T, int VEC, int ROWS> struct RecurrenceGradOp {
     resets.load(flags, w);
   }
   __device__ __forceinline__ void prep(Map<VEC> &m) {
-    float s[VEC], f[SEG][VEC], least[ROWS];
+    float h[VEC], f[SEG][VEC], least[ROWS];
     flags.bits(cut);
     keep_behind<T, VEC>(gv, n);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) least[j] = kTiny;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) s[j] = mark[j];
+    for (int j = 0; j < VEC; ++j) h[j] = mark[j];
 #pragma unroll
     for (int i = 0; i < SEG; ++i) {
       dv[i] = dn[i];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        sigmoid2(gv[i][j], f[i][j], q[i][j]);
-        const float v = xv[i][j], p = (cut[ROWS == 1 ? 0 : j] >> i) & 1 ? 0.f : s[j];
-        s[j] = fmaf(f[i][j], p, q[i][j] * v);
-        w[i][j] = (p - v) * (f[i][j] * q[i][j]);
+        float q; s[i][j] = sigmoid2(gv[i][j], f[i][j], q);
+        const float v = xv[i][j], p = (cut[ROWS == 1 ? 0 : j] >> i) & 1 ? 0.f : h[j];
+        h[j] = fmaf(f[i][j], p, q * v);
+        w[i][j] = (p - v) * (f[i][j] * q);
       }
     }
 #pragma unroll
@@ -189,8 +190,9 @@ template <class T, int VEC, int ROWS> struct RecurrenceGradOp {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float G = dv[i][j] + E[j];
-        E[j] = (cut[ROWS == 1 ? 0 : j] >> i) & 1 ? 0.f : (1.f - q[i][j]) * G;
-        a[i][j] = q[i][j] * G; w[i][j] *= G;
+        float f, q; sigmoid_again(s[i][j], f, q);
+        E[j] = (cut[ROWS == 1 ? 0 : j] >> i) & 1 ? 0.f : f * G;
+        a[i][j] = q * G; w[i][j] *= G;
       }
     }
     write_steps<T, VEC>(dx, at, a);

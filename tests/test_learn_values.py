@@ -1,8 +1,10 @@
 """agarcl_amd.learn on the GPU where an error would hide: policies that are NaN, small forget factors, upstream gradients that are not plain numbers in memory, what becomes
 of the outputs afterwards.  Tolerances in units of E = 2^-24, on top of those of test_learn_ops.py."""
-
 import pytest
 import torch
+
+import learn_formulas as F
+from learn_formulas import E, d, near
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +87,55 @@ def test_a_nan_move_is_not_a_move(learn, V, what):
     assert all(torch.equal(s[rest], t[rest]) for s, t in zip(a, good))
     p["mean"], p["log_std"], p["normal"] = torch.tensor([[inf, -inf]]).repeat(9, 1), torch.zeros(9, 2), torch.zeros(9, 2)
     assert learn.sample_actions(**{k: t.cuda() for k, t in p.items()}).move.tolist() == [[1.0, -1.0]] * 9
+
+
+# ---- small forget factors -------------------------------------------------------------------------------------------------------------------------
+# All gradients that come in are >= 0, so no sum cancels: every step a gradient crosses multiplies it by f, relative error (6 + 1.5 G) E with G = 16, and adds the next, 3 E more: 33 E.
+# Every 21 steps a gradient comes in anew, and what is older has crossed three factors of e^-8 or less since: it is not seen beside it.  So a total gradient has crossed at most 21
+# steps with its own step's, 22 x 33 E, and the joins' 64 E of any length: 790 E, relative.  dx multiplies by 1 - f (30 E + 1 rounding), dgate by f, 1 - f and p - x; p is good to
+# (12 + 3 G + 64 + 3 / min(1 - f)) E <= 150 E (gates are 2 at most) with x <= 1.
+
+def small_factors(T, rows, C, dtype, dh_too):
+    g = rng(T + C)
+    t, c = torch.arange(T)[:, None], torch.arange(C)[None]
+    gate = torch.where((t + c // 5) % 7 == 3, -(8.0 + 2 * (c % 5)), torch.full((), 2.0))
+    gate = gate[:, None, :].expand(T, rows, C).contiguous()
+    x = ((torch.rand(T, rows, C, generator=g) + 1) / 2) * torch.where(torch.rand(T, rows, C, generator=g) < 0.5, -1.0, 1.0)
+    dh = torch.zeros(T, rows, C)
+    if dh_too:
+        dh[T % 21::21] = torch.rand(dh[T % 21::21].shape, generator=g) + 0.5
+    return x.to(dtype), gate.to(dtype), torch.rand(rows, C, generator=g), dh.to(dtype), torch.rand(rows, C, generator=g) + 0.5
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("C", [35, 70])
+@pytest.mark.parametrize("T,rows,resets", [(5, 1, False), (13, 3, False), (21, 1, True), (7, 2000, False), (20, 4000, True), (2003, 1, False), (3001, 2, True)])
+def test_gradients_through_small_forget_factors(learn, T, rows, C, resets, dtype):
+    x, gate, state, dh, dlast = (t.cuda() for t in small_factors(T, rows, C, dtype, T > 21))
+    reset = None
+    if resets:
+        reset = torch.zeros(T, rows, dtype=torch.bool)
+        reset[T // 2::10] = True
+        reset = reset.cuda()
+    leaves = [t.clone().requires_grad_() for t in (x, gate, state)]
+    h, last = learn.gated_recurrence(*leaves, reset)
+    dx, dgate, dstate = torch.autograd.grad((h, last), leaves, (dh, dlast))
+    x, gate, G, dh = d(x), d(gate), d(dlast), d(dh)
+    f, q = torch.sigmoid(gate), torch.sigmoid(-gate)
+    seen, s = [], d(state)
+    for t in range(T):
+        p = s if reset is None else torch.where(F.flags(reset)[t][:, None], 0.0, s)
+        seen.append(p)
+        s = f[t] * p + q[t] * x[t]
+    want = [torch.empty_like(x), torch.empty_like(x)]
+    room = torch.empty_like(x)
+    for t in range(T - 1, -1, -1):
+        G = G + dh[t]
+        want[0][t], want[1][t] = q[t] * G, G * (seen[t] - x[t]) * f[t] * q[t]
+        room[t] = G * f[t] * q[t] * ((seen[t] - x[t]).abs() * 860 + 160) * E
+        G = f[t] * G
+        if reset is not None:
+            G = torch.where(F.flags(reset)[t][:, None], 0.0, G)
+    near(dx, want[0], want[0] * 830 * E, "dx")
+    near(dgate, want[1], room, "dgate")
+    near(dstate, G, G * 800 * E, "dstate")
