@@ -418,7 +418,10 @@ __global__ __launch_bounds__(512) void k_loss_stats(const agarcl_policy_loss_arg
   a.loss[0] = (float)((kl - sums[1] - ent) * by);
   for (int i = 1; i < 5; ++i) a.stats[i - 1] = (float)(sums[i] * inv);
   a.stats[4] = (float)sums[0]; a.stats[5] = a.stats[6] = a.stats[7] = 0.f;
-  if (a.dlog_std && !a.log_std_per_row) for (int d = 0; d < 2; ++d) ((float *)a.dlog_std)[d] = (float)(sums[5 + d] * by);
+  if (a.dlog_std && !a.log_std_per_row) {
+    const double up = a.upstream ? (double)*a.upstream : 1.;
+    for (int d = 0; d < 2; ++d) ((float *)a.dlog_std)[d] = (float)(sums[5 + d] * by * up);
+  }
 }
 
 // How many kinds call for which kernel.  What a row needs besides its kinds (a logarithm, exponentials, the sums over its lanes) is a few hundred instructions of every

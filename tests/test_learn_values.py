@@ -1,5 +1,7 @@
 """agarcl_amd.learn on the GPU where an error would hide: policies that are NaN, small forget factors, upstream gradients that are not plain numbers in memory, what becomes
 of the outputs afterwards.  Tolerances in units of E = 2^-24, on top of those of test_learn_ops.py."""
+import ctypes
+
 import pytest
 import torch
 
@@ -139,3 +141,37 @@ def test_gradients_through_small_forget_factors(learn, T, rows, C, resets, dtype
     near(dx, want[0], want[0] * 830 * E, "dx")
     near(dgate, want[1], room, "dgate")
     near(dstate, G, G * 800 * E, "dstate")
+
+
+# ---- the gradient of the loss itself ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("per_row", [0, 1])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_c_entry_multiplies_every_gradient_by_upstream(learn, per_row, weighted):
+    """one call for loss and gradients (the autograd node makes two): a power of two as the upstream gradient is exact in all of them"""
+    from agarcl_amd import _capi
+    lib = _capi.hip_lib()
+    R, V, g = 300, 5, rng(4)
+    t = dict(logits=torch.randn(R, V, generator=g), mean=torch.randn(R, 2, generator=g), log_std=torch.randn(R, 2, generator=g) * 0.3 if per_row else torch.tensor([-0.5, 0.2]),
+             move=torch.randn(R, 2, generator=g), old_log_prob=torch.full((R,), -4.0), advantage=torch.randn(R, generator=g), kind=torch.randint(0, V, (R,), generator=g).int())
+    if weighted:
+        t["weight"] = torch.rand(R, generator=g)
+    t = {k: v.cuda() for k, v in t.items()}
+    results = []
+    for up in (None, 1.0, 0.25, 1024.0):
+        out = dict(loss=torch.zeros(1), stats=torch.zeros(8), dlogits=torch.zeros(R, V), dmean=torch.zeros(R, 2), dlog_std=torch.zeros(R, 2) if per_row else torch.zeros(2))
+        out = {k: v.cuda() for k, v in out.items()}
+        upstream = None if up is None else torch.tensor([up], device="cuda")
+        work = torch.empty(lib.agarcl_policy_loss_work(), dtype=torch.float64, device="cuda")
+        a = _capi.PolicyLossArgs(rows=R, kinds=V, dtype=0, device=0, logits_stride=V, log_std_per_row=per_row, mean_over_weight=1, clip_low=0.2, clip_high=0.2, kl_coef=0.1, entropy_coef=0.01,
+                                 want_stats=1, work=work.data_ptr(), upstream=None if up is None else upstream.data_ptr(), stream=torch.cuda.current_stream().cuda_stream,
+                                 **{k: v.data_ptr() for k, v in dict(t, **out).items()})
+        assert lib.agarcl_policy_loss(ctypes.byref(a)) == 0, lib.agarcl_learn_error()
+        torch.cuda.synchronize()
+        results.append((up or 1.0, out))
+    one = results[0][1]
+    assert one["dlog_std"].abs().min() > 0
+    for up, out in results[1:]:
+        assert torch.equal(out["loss"], one["loss"]) and torch.equal(out["stats"], one["stats"])
+        for k in ("dlogits", "dmean", "dlog_std"):
+            assert torch.equal(out[k], one[k] * up), (k, up)
