@@ -31,10 +31,12 @@ void done(int rc) {
 
 // ---- arguments ------------------------------------------------------------------------------------------------------------------------------
 std::string shape_text(at::IntArrayRef s) { std::string t = "("; for (size_t i = 0; i < s.size(); ++i) t += (i ? ", " : "") + std::to_string(s[i]); return t + (s.size() == 1 ? ",)" : ")"); }
+// t with its numbers in memory as they are (a view that negates when it is read lies there with the other sign)
+Tensor stored(const Tensor &t) { return t.defined() ? t.resolve_neg() : t; }
 Tensor taken(py::handle h, const char *name) {
   const Tensor &t = THPVariable_Unpack(h.ptr());
   if (t._fw_grad(0).defined()) refuse(std::string(name) + " carries a forward-mode gradient: there are none through these operators");      // (better said than lost)
-  return t.resolve_neg();      // (a view that negates when it is read: what stands in memory is not what it says)
+  return stored(t);
 }
 Tensor optional(py::handle h, const char *name) {      // undefined for None
   if (h.is_none()) return {};
@@ -159,8 +161,8 @@ struct RecurrenceNode : torch::autograd::Node {
     no_second_gradient();
     if (!up[0].defined() && !up[1].defined()) return variable_list(3);
     const Tensor x = x_.unpack(), gate = gate_.unpack(), reset = reset_.unpack(), marks = marks_.unpack();
-    const Strided xs = steps(x), gs = steps(gate), rs = steps(reset), ds = steps(up[0]);
-    const Tensor dlast = whole(up[1]);
+    const Strided xs = steps(x), gs = steps(gate), rs = steps(reset), ds = steps(stored(up[0]));
+    const Tensor dlast = whole(stored(up[1]));
     agarcl_recurrence_args a = recurrence_args(x, x.sizes(), xs, gs, rs);
     Tensor dx = make(x.sizes(), x.scalar_type(), x), dgate = make(x.sizes(), x.scalar_type(), x), dstate = floats(x.sizes().slice(1), x);
     const Tensor work = scratch(agarcl_recurrence_work(a.steps, a.rows, a.width), x);
@@ -367,7 +369,7 @@ struct PolicyLossNode : torch::autograd::Node {
                  c.over, c.per_row, {c.need[0], c.need[1], c.need[2]}, results};
     std::vector<Tensor> kept;
     agarcl_policy_loss_args a = loss_args(logits, mean, log_std, now, kept);
-    const Tensor upstream = up[0].to(at::kFloat).contiguous();
+    const Tensor upstream = stored(up[0]).to(at::kFloat).contiguous();
     Tensor g[3];
     if (ahead && !capturing(logits)) {
       a.skip_if_one = 1; ahead = false;

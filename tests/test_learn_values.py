@@ -175,3 +175,45 @@ def test_c_entry_multiplies_every_gradient_by_upstream(learn, per_row, weighted)
         assert torch.equal(out["loss"], one["loss"]) and torch.equal(out["stats"], one["stats"])
         for k in ("dlogits", "dmean", "dlog_std"):
             assert torch.equal(out[k], one[k] * up), (k, up)
+
+
+def loss_call(learn, R=40, V=5):
+    g = rng(6)
+    t = [torch.randn(R, V, generator=g), torch.randint(0, V, (R,), generator=g).int(), torch.full((R,), -4.0), torch.randn(R, generator=g), torch.randn(R, 2, generator=g), torch.tensor([-0.5, 0.2]),
+         torch.randn(R, 2, generator=g)]
+    t = [k.cuda() for k in t]
+    for i in (0, 4, 5):
+        t[i].requires_grad_()
+    return [t[0], t[4], t[5]], lambda: learn.policy_loss(*t).loss
+
+
+def negated(t):
+    """t's numbers in a tensor that lies in memory with the other sign"""
+    t = torch._neg_view(-t)
+    assert t.is_neg()
+    return t
+
+
+def test_an_upstream_gradient_that_negates(learn):
+    leaves, loss = loss_call(learn)
+    for up in (1.0, 0.5):
+        up = torch.tensor(up, device="cuda")
+        want = torch.autograd.grad(loss(), leaves, up)
+        out = loss()
+        for _ in range(2):                                   # the gradients made ahead, and those of a second pass
+            got = torch.autograd.grad(out, leaves, negated(up), retain_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    out = loss()
+    through = (torch.complex(torch.zeros_like(out), out).conj() * 1j).real      # = out: autograd hands on a view that negates by itself
+    got, want = torch.autograd.grad(through, leaves), torch.autograd.grad(loss(), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_an_upstream_gradient_of_the_memory_that_negates(learn):
+    g = rng(7)
+    x, gate, state, dh, dlast = (torch.randn(*s, generator=g).cuda() for s in ((30, 4, 6), (30, 4, 6), (4, 6), (30, 4, 6), (4, 6)))
+    leaves = [t.requires_grad_() for t in (x, gate, state)]
+    want = torch.autograd.grad(learn.gated_recurrence(*leaves), leaves, (dh, dlast))
+    for a, b in ((negated(dh), dlast), (dh, negated(dlast)), (negated(dh), negated(dlast))):
+        got = torch.autograd.grad(learn.gated_recurrence(*leaves), leaves, (a, b))
+        assert all(torch.equal(s, t) for s, t in zip(got, want))
