@@ -31,8 +31,9 @@ void done(int rc) {
 
 // ---- arguments ------------------------------------------------------------------------------------------------------------------------------
 std::string shape_text(at::IntArrayRef s) { std::string t = "("; for (size_t i = 0; i < s.size(); ++i) t += (i ? ", " : "") + std::to_string(s[i]); return t + (s.size() == 1 ? ",)" : ")"); }
-// t with its numbers in memory as they are (a view that negates when it is read lies there with the other sign)
-Tensor stored(const Tensor &t) { return t.defined() ? t.resolve_neg() : t; }
+// t with its numbers in memory as they are: a view that negates when it is read lies there with the other sign, and torch's zeros without storage have a null address, which
+// says "none" to the C ABI
+Tensor stored(const Tensor &t) { return !t.defined() ? t : t._is_zerotensor() ? t.clone() : t.resolve_neg(); }
 Tensor taken(py::handle h, const char *name) {
   const Tensor &t = THPVariable_Unpack(h.ptr());
   if (t._fw_grad(0).defined()) refuse(std::string(name) + " carries a forward-mode gradient: there are none through these operators");      // (better said than lost)

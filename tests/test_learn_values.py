@@ -217,3 +217,33 @@ def test_an_upstream_gradient_of_the_memory_that_negates(learn):
     for a, b in ((negated(dh), dlast), (dh, negated(dlast)), (negated(dh), negated(dlast))):
         got = torch.autograd.grad(learn.gated_recurrence(*leaves), leaves, (a, b))
         assert all(torch.equal(s, t) for s, t in zip(got, want))
+
+
+# ---- tensors without memory -------------------------------------------------------------------------------------------------------------------------
+
+def zeros_unstored(*shape, dtype=torch.float32):
+    """zeros as autograd makes them where it need not store them: their address is null"""
+    t = torch._efficientzerotensor(shape, dtype=dtype, device="cuda")
+    assert t._is_zerotensor()
+    return t
+
+
+def test_zeros_that_are_not_stored(learn):
+    leaves, loss = loss_call(learn)
+    for _ in range(2):
+        out = loss()
+        for _ in range(2):
+            got = torch.autograd.grad(out, leaves, zeros_unstored(), retain_graph=True)
+            assert all((t == 0).all() for t in got)
+    g = rng(8)
+    x, gate, state = (torch.randn(*s, generator=g).cuda().requires_grad_() for s in ((9, 4, 6), (9, 4, 6), (4, 6)))
+    want = torch.autograd.grad(learn.gated_recurrence(x, gate, state), (x, gate, state), (torch.ones(9, 4, 6, device="cuda"), torch.zeros(4, 6, device="cuda")))
+    got = torch.autograd.grad(learn.gated_recurrence(x, gate, state), (x, gate, state), (torch.ones(9, 4, 6, device="cuda"), zeros_unstored(4, 6)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    z, kind, old, adv = torch.randn(9, 3, generator=g).cuda(), torch.zeros(9, dtype=torch.int32, device="cuda"), torch.full((9,), -1.0, device="cuda"), torch.randn(9, generator=g).cuda()
+    for name, dtype, shape in (("ref_log_prob", torch.float32, (9,)), ("weight", torch.float32, (9,)), ("allowed", torch.bool, (9, 3))):
+        a = learn.policy_loss(z, kind, old, adv, kl_coef=0.1, **{name: zeros_unstored(*shape, dtype=dtype)})
+        b = learn.policy_loss(z, kind, old, adv, kl_coef=0.1, **{name: torch.zeros(*shape, dtype=dtype, device="cuda")})
+        assert all(torch.equal(s, t) for s, t in zip(a, b)), name
+    got = learn.sample_actions(z, allowed=zeros_unstored(9, 3, dtype=torch.bool))
+    assert (got.kind == 0).all() and (got.log_prob == 0).all()
