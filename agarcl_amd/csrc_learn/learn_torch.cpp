@@ -89,9 +89,9 @@ int64_t product(at::IntArrayRef s) { int64_t n = 1; for (auto k : s) n *= k; ret
 const void *ptr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void *out(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor &ref) { return at::detail::empty_cuda(shape, type, ref.device(), std::nullopt); }      // (at::empty takes a microsecond)
-// a tensor of its own on a part of another's memory, `at` elements behind its beginning: an allocation and its share of the host's time less
-Tensor part(const Tensor &of, int64_t at, at::IntArrayRef shape, at::ScalarType type) {
-  auto t = c10::make_intrusive<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(of.storage()), of.key_set(), c10::scalarTypeToTypeMeta(type));
+// a tensor of its own on a part of another's memory, `at` elements behind its beginning and of its type: an allocation and its share of the host's time less
+Tensor part(const Tensor &of, int64_t at, at::IntArrayRef shape) {
+  auto t = c10::make_intrusive<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(of.storage()), of.key_set(), of.dtype());
   t->set_storage_offset(at);
   t->set_sizes_contiguous(shape);
   return Tensor(std::move(t));
@@ -289,9 +289,10 @@ py::tuple sample_actions(py::handle hlogits, py::handle hmean, py::handle hstd, 
   a.logits = ptr(z.t); a.logits_stride = z.stride; a.allowed = (const uint8_t *)ptr(k.t); a.allowed_stride = k.stride; a.gumbel = (const float *)ptr(g.t); a.gumbel_stride = g.stride;
   a.mean = ptr(m); a.log_std = ptr(s); a.log_std_per_row = per_row; a.normal = (const float *)ptr(n);
   const int64_t moves = mean.defined() ? 2 * a.rows : 0;
-  const Tensor all = floats({2 * moves + 2 * a.rows}, logits), kind = part(all, 2 * moves, lead, at::kInt), log_prob = part(all, 2 * moves + a.rows, lead, at::kFloat);
+  // (kind has an allocation of its own: torch does not save or copy tensors together that share their memory and differ in type)
+  const Tensor all = floats({2 * moves + a.rows}, logits), kind = make(lead, at::kInt, logits), log_prob = part(all, 2 * moves, lead);
   Tensor raw, move;
-  if (mean.defined()) { raw = part(all, 0, mean.sizes(), at::kFloat); move = part(all, moves, mean.sizes(), at::kFloat); }
+  if (mean.defined()) { raw = part(all, 0, mean.sizes()); move = part(all, moves, mean.sizes()); }
   a.kind = (int32_t *)out(kind); a.log_prob = (float *)out(log_prob); a.raw = (float *)out(raw); a.move = (float *)out(move); a.stream = stream_of(logits);
   done(agarcl_sample_actions(&a));
   return mean.defined() ? py::make_tuple(move, kind, log_prob, raw) : py::make_tuple(py::none(), kind, log_prob, py::none());
@@ -419,7 +420,7 @@ py::tuple policy_loss(py::handle hlogits, py::handle hkind, py::handle hold, py:
     }
     node->keep(logits, mean, log_std, c);
   } else loss_forward(logits, mean, log_std, c, {}, false);
-  const auto number = [&](int i) { return part(c.results, i, {}, at::kFloat); };
+  const auto number = [&](int i) { return part(c.results, i, {}); };
   const Tensor loss = number(kLoss);
   if (node) torch::autograd::set_history(loss, node);
   return py::make_tuple(loss, number(kStats), number(kStats + 1), number(kStats + 2), number(kStats + 3));

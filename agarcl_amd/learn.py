@@ -79,7 +79,7 @@ def sample_actions(logits, mean=None, log_std=None, gumbel=None, normal=None, al
 
     Returns Actions(move, kind, log_prob, raw): `venv.step(actions)` takes it as it is.  kind int32 = the lowest index of the largest logits + gumbel
     among the allowed (0, "none", where nothing is allowed); raw = mean + exp(log_std) * normal; move = raw limited to [-1, 1]; log_prob of (kind, raw):
-    what policy_loss divides by.  A logit of -inf is not allowed.  Without gradients.  The four lie in one allocation (clone() what is to be kept alone)."""
+    what policy_loss divides by.  A logit of -inf is not allowed.  Without gradients.  log_prob, raw and move lie in one allocation (clone() what is to be kept alone)."""
     return Actions._make(_learn.sample_actions(logits, mean, log_std, gumbel, normal, allowed))
 
 

@@ -1,6 +1,7 @@
 """agarcl_amd.learn on the GPU where an error would hide: policies that are NaN, small forget factors, upstream gradients that are not plain numbers in memory, what becomes
 of the outputs afterwards.  Tolerances in units of E = 2^-24, on top of those of test_learn_ops.py."""
 import ctypes
+import io
 
 import pytest
 import torch
@@ -247,3 +248,20 @@ def test_zeros_that_are_not_stored(learn):
         assert all(torch.equal(s, t) for s, t in zip(a, b)), name
     got = learn.sample_actions(z, allowed=zeros_unstored(9, 3, dtype=torch.bool))
     assert (got.kind == 0).all() and (got.log_prob == 0).all()
+
+
+# ---- what becomes of the outputs ----------------------------------------------------------------------------------------------------------------------
+
+def test_actions_are_saved_and_copied_together(learn):
+    import copy
+    a = learn.sample_actions(torch.randn(50, 3, generator=rng(9)).cuda(), torch.zeros(50, 2, device="cuda"), torch.zeros(2, device="cuda"))
+    f = io.BytesIO()
+    torch.save(dict(a._asdict()), f)
+    f.seek(0)
+    back = torch.load(f, weights_only=True)
+    assert all(torch.equal(back[k], t) and back[k].dtype == t.dtype for k, t in a._asdict().items())
+    twin = copy.deepcopy(dict(a._asdict()))
+    assert all(torch.equal(twin[k], t) and twin[k].dtype == t.dtype for k, t in a._asdict().items())
+    alone = learn.sample_actions(torch.zeros(4, 3, device="cuda"))
+    f = io.BytesIO()
+    torch.save([alone.kind, alone.log_prob], f)
