@@ -15,7 +15,8 @@ the host or waits for the GPU, so all of it can be captured into a graph.
     h, _ = learn.gated_recurrence(x, gate, memory_at_start, reset)           # [T, N, C]; reset[t] = ended of step t - 1
     loss = learn.policy_loss(logits, kinds, log_probs, advantage, mean, log_std, raws).loss           # + the value loss, then backward()
 
-Conventions of every function: tensors live on one GPU; a rollout's first axis is time, then the arenas (and agents); `x`, `gate`, `logits`, `mean`,
+Conventions of every function: tensors live on one GPU; a rollout's first axis is time, then the arenas (and agents: venv's info["ended"] is per arena, so for
+[N, agents] the resets are info["ended"][:, None].expand(N, agents)); `x`, `gate`, `logits`, `mean`,
 `value` are float32, bfloat16 or float16, everything that counts, sums or carries a state is float32; flags are bool or uint8.  A wrong argument raises
 ValueError, a failing call AgarclError.  Kernels run on the current stream of the tensors' device, also when that is not the current device.
 Tensors of other strides than a kernel reads are copied first (a step's slice, a row, has to be contiguous; steps and rows may lie apart).  There are no

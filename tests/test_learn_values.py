@@ -265,3 +265,41 @@ def test_actions_are_saved_and_copied_together(learn):
     alone = learn.sample_actions(torch.zeros(4, 3, device="cuda"))
     f = io.BytesIO()
     torch.save([alone.kind, alone.log_prob], f)
+
+
+# ---- several agents -----------------------------------------------------------------------------------------------------------------------------------
+
+def test_acting_with_several_agents(learn):
+    """rows are arenas x agents; info["ended"] is the arenas' and goes to their agents"""
+    from agarcl_amd.vector_env import AgarioVectorEnv
+    N, n, T, C = 6, 2, 14, 8
+    venv = AgarioVectorEnv(N, obs_type="ram", arena_size=200, num_pellets=200, num_viruses=4, num_agents=n, multi_agent=True, number_steps=5)
+    D = venv.single_observation_shape[-1]
+    g = torch.Generator(device="cuda")
+    g.manual_seed(0)
+    w = [torch.randn(s, generator=g, device="cuda") * 0.05 for s in ((D, C), (D, C), (C, 3), (C, 2), (C,))]
+    obs, _ = venv.reset(seed=1)
+    state, ended, xs, gs, hs, resets, rew, term, trunc, value = torch.zeros(N, n, C, device="cuda"), torch.zeros(N, dtype=torch.bool, device="cuda"), [], [], [], [], [], [], [], []
+    for t in range(T):
+        o = torch.tanh(obs * 0.05)
+        x, gate, reset = o @ w[0], o @ w[1], ended[:, None].expand(N, n)
+        h, state = learn.recurrence_step(x, gate, state, reset)
+        a = learn.sample_actions(h @ w[2], h @ w[3], torch.full((2,), -0.5, device="cuda"), normal=torch.randn(N, n, 2, generator=g, device="cuda"))
+        assert a.move.shape == (N, n, 2) and a.kind.shape == (N, n)
+        obs, reward, terminated, truncated, info = venv.step(a)
+        ended = info["ended"].clone()
+        for buf, v in ((xs, x), (gs, gate), (hs, h), (resets, reset), (rew, reward), (term, terminated), (trunc, truncated), (value, h @ w[4])):
+            buf.append(v.clone())
+    assert torch.stack(resets).any()
+    h, last = learn.gated_recurrence(torch.stack(xs), torch.stack(gs), None, torch.stack(resets))
+    M = max(t.abs().max().item() for t in xs)
+    assert max(t.abs().max().item() for t in gs) <= 4          # (what the bound assumes: (12 + 3 G + 64 + 3 T) E M, twice)
+    near(h, d(torch.stack(hs)), 2 * (12 + 12 + 64 + 3 * T) * E * M)
+    near(last, d(state), 2 * (12 + 12 + 64 + 3 * T) * E * M)
+    args = [torch.stack(t) for t in (rew, value)] + [state @ w[4], torch.stack(term), torch.stack(trunc)]
+    got = learn.advantages(*args)
+    flat = [t.cpu().reshape(t.shape[0], N * n) if t.dim() == 3 else t.cpu().reshape(N * n) for t in args]
+    want = F.advantages(*flat, None, float(torch.tensor(0.99)), float(torch.tensor(0.95)))
+    top = T * (args[0].abs().max().item() + 2 * args[1].abs().max().item() + args[2].abs().max().item())      # the largest advantage there can be
+    near(got.advantage.reshape(T, N * n), want[0], (6 + 2 * T + 64) * E * top)
+    venv.close()
