@@ -303,3 +303,41 @@ def test_acting_with_several_agents(learn):
     top = T * (args[0].abs().max().item() + 2 * args[1].abs().max().item() + args[2].abs().max().item())      # the largest advantage there can be
     near(got.advantage.reshape(T, N * n), want[0], (6 + 2 * T + 64) * E * top)
     venv.close()
+
+
+# ---- the gradient against differences -----------------------------------------------------------------------------------------------------------------
+
+def test_recurrence_gradient_against_differences(learn):
+    """each gradient for itself, along random directions, with room for what the formulas lose and no more: a gradient of 0 is farther off, which is asserted.
+    Crossing a step costs a total gradient (6 + 1.5 x 4 + 3) E of the sum of its terms' magnitudes: (21 x 15 + 64) E = 379 E in all (64 E for the joins); dx multiplies by 1 - f,
+    dgate by f, 1 - f and p - x (12 E and a rounding each), with p good to (12 + 12 + 64 + 3 x 21) E x 4 = 604 E.  Central differences with steps of 1e-6 in 64 bits: the third derivative
+    along v, |v| <= 4, of a product of 21 sigmoids is at most (21 x 4)^3 of the value's magnitude, 500: off by 5e-5; rounding by 1e-6."""
+    g = rng(11)
+    T, B, C = 21, 4, 6
+    x, gate, dh = (torch.randn(T, B, C, generator=g).clamp(-4, 4) for _ in range(3))
+    state, dlast = torch.randn(B, C, generator=g), torch.randn(B, C, generator=g)
+    reset = torch.rand(T, B, generator=g) < 0.1
+    leaves = [t.cuda().requires_grad_() for t in (x, gate, state)]
+    got = torch.autograd.grad(learn.gated_recurrence(*leaves, reset.cuda()), leaves, (dh.cuda(), dlast.cuda()))
+
+    def value(at):
+        h, last = F.recurrence(*at, reset)
+        return (h * d(dh)).sum() + (last * d(dlast)).sum()
+
+    f, q = torch.sigmoid(d(gate)), torch.sigmoid(-d(gate))
+    h, _ = F.recurrence(x, gate, state, reset)
+    G, off = d(dlast).abs(), [torch.empty_like(f), torch.empty_like(f), None]
+    for t in reversed(range(T)):
+        G = G + d(dh)[t].abs()
+        p = torch.where(reset[t][:, None], 0.0, h[t - 1] if t else d(state))
+        off[0][t], off[1][t] = q[t] * G * 392 * E, G * f[t] * q[t] * ((p - d(x)[t]).abs() * 410 + 604) * E
+        G = torch.where(reset[t][:, None], 0.0, f[t] * G)
+    off[2] = G * 380 * E
+    for i, name in enumerate(("dx", "dgate", "dstate")):
+        for k in range(3):
+            v = torch.randn(leaves[i].shape, generator=g, dtype=torch.float64).clamp(-4, 4)
+            shifted = [[d(t) + (s * v if j == i else 0) for j, t in enumerate((x, gate, state))] for s in (1e-6, -1e-6)]
+            want = (value(shifted[0]) - value(shifted[1])) / 2e-6
+            room = (off[i] * v.abs()).sum() + 1e-4
+            assert abs((d(got[i]) * v).sum() - want) < room, (name, k)
+            assert abs(want) > room, (name, k, "a gradient of 0 would pass")
