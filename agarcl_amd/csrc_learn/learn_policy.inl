@@ -99,7 +99,8 @@ template <class T> __device__ __forceinline__ void row_kind(const agarcl_policy_
 struct LossRow { float sg, c0, c1; };
 struct LossTotals { float inv; bool shared_std; };
 
-// e^x - 1 and e^x - 1 - x: near 0, where both are the difference of near numbers, from the series (|x| < 0.35: 2e-8 of the value is left out)
+// e^x - 1 and e^x - 1 - x: near 0, where both are the difference of near numbers, from the series (|x| < 0.35: of
+// e^x - 1 - x 1e-7 is left out, of e^x - 1 2e-8)
 __device__ __forceinline__ void exp_less(float x, float &less1, float &less1x) {
   const float p = fmaf(x, fmaf(x, fmaf(x, fmaf(x, fmaf(x, 1.f / 5040, 1.f / 720), 1.f / 120), 1.f / 24), 1.f / 6), 0.5f) * x * x, e = __expf(x) - 1.f;
   const bool near = fabsf(x) < 0.35f;
