@@ -14,8 +14,8 @@ DEPS = (sorted(glob.glob(os.path.join(HERE, "csrc", "*"))) + sorted(glob.glob(os
         + [os.path.join(HERE, "..", "include", h) for h in ("agarcl_batch.h", "agarcl_vec.h", "agarcl_learn.h")])
 OUT = os.path.join(HERE, "libagarcl_hip.so")
 
-# hipcc -O3 turns ordinary float code into packed f32 instructions, some forms of which have given wrong results on this hardware, without an error.  Without
-# them the engine is no slower either, us per step with / without: mode 6 at 4096 arenas 351 / 333, C1 90 / 85, task 3 99 / 96, C2 9.1 / 9.1
+# hipcc -O3 turns ordinary float code into packed f32 instructions, some forms of which have given wrong results on this hardware, without an error.  What
+# the engine takes with / without them, us per step at 4096 arenas: mode 6 351 / 333, C1 90 / 85, task 3 99 / 96, C2 9.1 / 9.1, 30 scripted bots 175 / 185
 NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 FLAGS = [
