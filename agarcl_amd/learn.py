@@ -80,7 +80,8 @@ def sample_actions(logits, mean=None, log_std=None, gumbel=None, normal=None, al
 
     Returns Actions(move, kind, log_prob, raw): `venv.step(actions)` takes it as it is.  kind int32 = the lowest index of the largest logits + gumbel
     among the allowed (0, "none", where nothing is allowed); raw = mean + exp(log_std) * normal; move = raw limited to [-1, 1]; log_prob of (kind, raw):
-    what policy_loss divides by.  A logit of -inf is not allowed.  Without gradients.  log_prob, raw and move lie in one allocation (clone() what is to be kept alone)."""
+    what policy_loss divides by.  A NaN stays one in raw, move and log_prob (an arena that is stepped with it holds it until its next reset).  A logit of
+    -inf is not allowed.  Without gradients.  log_prob, raw and move lie in one allocation (clone() what is to be kept alone)."""
     return Actions._make(_learn.sample_actions(logits, mean, log_std, gumbel, normal, allowed))
 
 
@@ -94,11 +95,16 @@ def policy_loss(logits, kind, old_log_prob, advantage, mean=None, log_std=None, 
 
     clip: a number, or (below, above).  ref_log_prob: the log-probability under a reference policy; old_log_prob without one.  reduction: "mean" (weighted;
     0 where the weights sum to 0) or "sum".  Returns PolicyLoss(loss, surrogate, kl, entropy, clipped): loss is differentiable in logits, mean and
-    log_std; the others are weighted means of min(..), of the KL term, of H and of "the clip took the gradient", without gradients.
+    log_std; the others are weighted means of min(..), of the KL term, of H and of "the clip took the gradient"
+    (r > 1 + above where A >= 0, r < 1 - below elsewhere), without gradients.
 
     A row is left out -- it adds nothing and its gradients are 0 -- where its weight is 0, its kind is outside 0 .. kinds - 1 (padding), or its kind is not
     allowed (a logit of -inf is not); except by its weight it still counts in the mean.  What stands in such rows and places is never used.
-    Gradients in float16: scale the loss (the upstream gradient is applied in float32, before the one rounding)."""
+    Gradients in float16: scale the loss (the upstream gradient is applied in float32, before the one rounding).
+
+    In float32 and bfloat16 the forward pass writes the gradients for an upstream gradient of 1 as well, and they are kept until the backward pass (the size of the
+    logits).  Where the upstream gradient is another -- a loss that is divided or scaled after this call -- the backward pass works them out once more, twice the
+    memory traffic in all: for many kinds let reduction="sum" and the weights hold the factor."""
     if reduction not in ("mean", "sum"):
         raise ValueError("reduction must be 'mean' or 'sum'")
     low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)

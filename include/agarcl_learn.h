@@ -77,7 +77,7 @@ int agarcl_advantages(const agarcl_advantages_args *a);
 /* The env's action: a kind out of `kinds` (agarcl_vec_step's act has 3) by logits, and -- where mean is given -- a move by two independent normal
  * distributions.  A kind is allowed unless allowed[row][kind] is 0 or its logit is -inf; what stands in a place that is not allowed is never used.
  *   kind = the lowest index of the largest logit + gumbel among the allowed (gumbel NULL: of the largest logit); 0 where nothing is allowed
- *   raw = mean + exp(log_std) normal (normal NULL: mean);  move = raw limited to [-1, 1], what the engine takes
+ *   raw = mean + exp(log_std) normal (normal NULL: mean);  move = raw limited to [-1, 1], what the engine takes; a NaN stays one, in log_prob too
  *   log_prob = log softmax(logits over the allowed)[kind] (0 where nothing is allowed) + the normal log-density of raw */
 typedef struct agarcl_sample_args {
   int64_t rows, kinds;
