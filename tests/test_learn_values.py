@@ -341,3 +341,28 @@ def test_recurrence_gradient_against_differences(learn):
             room = (off[i] * v.abs()).sum() + 1e-4
             assert abs((d(got[i]) * v).sum() - want) < room, (name, k)
             assert abs(want) > room, (name, k, "a gradient of 0 would pass")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("per_row", [False, True])
+def test_gradients_of_some_of_the_leaves(learn, per_row, dtype):
+    """whatever is differentiated, each gradient is what it is beside the others, for an upstream gradient of 1 and another, the first time and the second"""
+    R, V, g = 70, 9, rng(12)
+    t = dict(logits=torch.randn(R, V, generator=g).to(dtype), mean=torch.randn(R, 2, generator=g).to(dtype),
+             log_std=(torch.randn(R, 2, generator=g) * 0.3).to(dtype) if per_row else torch.tensor([-0.5, 0.2]))
+    fixed = dict(kind=torch.randint(-1, V + 1, (R,), generator=g).int(), old_log_prob=torch.full((R,), -4.0), advantage=torch.randn(R, generator=g), move=torch.randn(R, 2, generator=g),
+                 weight=torch.rand(R, generator=g))
+    t, fixed = ({k: v.cuda() for k, v in s.items()} for s in (t, fixed))
+    for up in (1.0, 8.0):
+        up = torch.tensor(up, device="cuda")
+        results = {}
+        for wanted in (("logits", "mean", "log_std"), ("logits",), ("mean",), ("log_std",), ("logits", "log_std"), ("mean", "log_std"), ("logits", "mean")):
+            leaves = {k: v.detach().requires_grad_(k in wanted) for k, v in t.items()}
+            out = learn.policy_loss(**leaves, **fixed, kl_coef=0.1, entropy_coef=0.01)
+            for again in (False, True):
+                for k, got in zip(wanted, torch.autograd.grad(out.loss, [leaves[k] for k in wanted], up, retain_graph=True)):
+                    want = results.setdefault(k, got)
+                    if again:      # (the weights' sum is rounded to 32 bits between the passes, a shared log_std's gradient before it is multiplied)
+                        near(got, d(want), d(want).abs() * (4 * E + F.HALF[got.dtype]), k)
+                    else:
+                        assert torch.equal(got, want), (k, wanted)
