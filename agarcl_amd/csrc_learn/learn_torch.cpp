@@ -86,7 +86,12 @@ void capture_reaches(const Tensor &ref, std::initializer_list<const Tensor *> in
   }
 }
 int64_t product(at::IntArrayRef s) { int64_t n = 1; for (auto k : s) n *= k; return n; }
-const void *ptr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+const void *ptr(const Tensor &t) {
+  if (!t.defined()) return nullptr;
+  const void *p = t.const_data_ptr();
+  if (!p && t.numel()) refuse("a tensor without memory of its own (a wrapper's, a fake one)");      // (null says "none" to the C ABI)
+  return p;
+}
 void *out(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor make(at::IntArrayRef shape, at::ScalarType type, const Tensor &ref) { return at::detail::empty_cuda(shape, type, ref.device(), std::nullopt); }      // (at::empty takes a microsecond)
 // a tensor of its own on a part of another's memory, `at` elements behind its beginning and of its type: an allocation and its share of the host's time less

@@ -250,6 +250,30 @@ def test_zeros_that_are_not_stored(learn):
     assert (got.kind == 0).all() and (got.log_prob == 0).all()
 
 
+class Wrapper(torch.Tensor):
+    """a tensor that is a tensor only to Python, as tensor subclasses that hold others are"""
+    @staticmethod
+    def __new__(cls, like):
+        return torch.Tensor._make_wrapper_subclass(cls, like.shape, dtype=like.dtype, device=like.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, *args):
+        raise AssertionError("nothing is computed with it")
+
+
+def test_tensors_without_memory_are_refused(learn):
+    z = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device="cuda")        # noqa: E731
+    loss = dict(logits=z(4, 3), kind=z(4, dtype=torch.int32), old_log_prob=z(4), advantage=z(4), ref_log_prob=z(4), allowed=z(4, 3, dtype=torch.bool), weight=z(4))
+    memory = dict(x=z(5, 4, 3), gate=z(5, 4, 3), state=z(4, 3), reset=z(5, 4, dtype=torch.bool))
+    rollout = dict(reward=z(5, 4), value=z(5, 4), next_value=z(4), terminated=z(5, 4, dtype=torch.bool), truncated=z(5, 4, dtype=torch.bool), final_value=z(5, 4))
+    acting = dict(logits=z(4, 3), gumbel=z(4, 3), allowed=z(4, 3, dtype=torch.bool), mean=z(4, 2), log_std=z(2), normal=z(4, 2))
+    for name, args in (("policy_loss", loss), ("gated_recurrence", memory), ("advantages", rollout), ("sample_actions", acting)):
+        getattr(learn, name)(**args)
+        for k in args:
+            with pytest.raises((ValueError, RuntimeError), match="memory of its own"):
+                getattr(learn, name)(**dict(args, **{k: Wrapper(args[k])}))
+
+
 # ---- what becomes of the outputs ----------------------------------------------------------------------------------------------------------------------
 
 def test_actions_are_saved_and_copied_together(learn):
