@@ -2,8 +2,8 @@
 //
 // Both are one pass over the logits: a row is in registers (or, beyond 8192 kinds, read twice) while its maximum, the sum s of e^(z - max) and
 // u = sum of e^(z - max) (z - max) are taken; log s and u / s give the log-probabilities and the entropy, and the gradient is written from the same registers:
-// reading the logits once and writing their gradient once is all the memory traffic there has to be (8209 rows of 6144 bf16, masked, with all gradients: 252 MB in 61 us,
-// 4.1 TB/s, where a large copy reaches 4.76: two exps and a dozen other instructions per kind stand beside it).  Up to 8 kinds a row is one thread's, up to 2048
+// reading the logits once and writing their gradient once is all the memory traffic there has to be (8209 rows of 6144 bf16, masked, with all gradients: 252 MB in 64 us,
+// 3.9 TB/s, where a large copy reaches 4.76: two exps and a dozen other instructions per kind stand beside it).  Up to 8 kinds a row is one thread's, up to 2048
 // a group of 1 to 64 lanes', beyond that a workgroup's.
 
 static const int kUnits = 256;      // compute units of an MI355X
