@@ -21,7 +21,8 @@ Conventions of every function: tensors live on one GPU; a rollout's first axis i
 ValueError, a failing call AgarclError.  Kernels run on the current stream of the tensors' device, also when that is not the current device.
 Tensors of other strides than a kernel reads are copied first (a step's slice, a row, has to be contiguous; steps and rows may lie apart).  There are no
 gradients of gradients: a backward pass with create_graph raises RuntimeError, a forward-mode gradient ValueError.  Forward and backward pass are captured
-together, with no eager graph of the same leaves alive: autograd would tie its stream to the capture (such a call raises ValueError).  An eager backward
+together, with no eager graph of the same leaves alive: autograd would tie its stream to the capture (such a call raises ValueError; a kept loss of a warm-up is
+such a graph, and torch.cuda.make_graphed_callables keeps one).  An eager backward
 pass is handed to a thread of autograd's and back, which takes longer than the kernels here: torch.autograd.set_multithreading_enabled(False) around it keeps
 it in the calling thread (the loss of 32768 rows with its gradients 37 us instead of 64)."""
 import collections
